@@ -1,0 +1,335 @@
+// The paged cache: tokens quantised as they are written, and read back.
+//
+// Both are one pass over the data and bound by its bytes. Eight elements of a row belong to one lane (16 bytes of
+// fp16), D / 8 lanes to a row. int8: the row's largest magnitude `top` by shuffles, scale = top / 127, code =
+// rint((127 x) / top): for fp16 inputs 127 x is exact in float32 and the quotient of two 18- and 11-bit integers never
+// comes closer to a half without being one than float32 resolves, so every code is the correctly rounded one.
+// A block of the append owns one page of one (sequence, head): it alone writes the page's minimum of phi.
+#include "fpa_serve.h"
+
+namespace fpa {
+namespace {
+
+constexpr int kThreads = 128;
+
+// Eight consecutive elements of a row in float32.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t stride, bool vec, float (&x)[8]) {
+  if (vec) {
+    if constexpr (sizeof(T) == 2) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(h[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i * stride]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    uint4 w;
+    __half2* h = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = w;
+  } else {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+struct Str3 {
+  int64_t b, h, t;
+};
+
+struct AppendParams {
+  CacheView c;
+  const void* src[2];  // k, v
+  Str4 st[2];
+  int vec[2];          // rows can be read 16 bytes at a time
+  const float* phi;
+  const float* psi;
+  Str3 sphi, spsi;
+  const int32_t* table;
+  int64_t table_stride;
+  int max_pages, n;
+  const int32_t* start;
+  const int32_t* counts;
+};
+
+// T: type of k and v; kInt8: codes and scales, else rows as they are.
+template <typename T, bool kInt8>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const CacheView& c = p.c;
+  const int h = blockIdx.y, b = blockIdx.z, page = 1 << c.page_shift;
+  const int start = p.start[b];
+  const int count = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+  if (count == 0) return;
+  const int64_t cap = int64_t(p.max_pages) << c.page_shift;
+  if (start < 0 || start >= cap) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) report_bad_page(c.status, kSiteAppend);
+    return;
+  }
+  // This block's page of the sequence and the tokens [i0, i1) that fall into it.
+  const int64_t pg = int64_t(start >> c.page_shift) + blockIdx.x;
+  const int64_t first = pg << c.page_shift;
+  const int i0 = int(max(first - start, int64_t(0))), i1 = int(min(first + page - start, int64_t(count)));
+  if (i0 >= i1) return;
+  const int pid = pg < p.max_pages ? p.table[b * p.table_stride + pg] : -1;
+  if (unsigned(pid) >= unsigned(c.n_pages)) {
+    if (threadIdx.x == 0) report_bad_page(c.status, kSiteAppend);
+    return;
+  }
+  const int64_t base = (int64_t(pid) * c.H + h) << c.page_shift;  // pool index of the page's slot 0
+  const int slot0 = int(start + i0 - first);
+  const int lanes = c.D >> 3, rows = kThreads / lanes;
+  const int sub = threadIdx.x / lanes, e0 = (threadIdx.x - sub * lanes) * 8;
+  const int tokens = i1 - i0;
+  // Rows 0 .. tokens - 1 are K's, the rest V's. Whole warps stay in the loop for the shuffles.
+  for (int r0 = 0; r0 < 2 * tokens; r0 += rows) {
+    const int r = r0 + sub;
+    const bool ok = r < 2 * tokens;
+    const int which = ok && r >= tokens ? 1 : 0, i = ok ? r - which * tokens : 0;
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    if (ok) {
+      const Str4& st = p.st[which];
+      load8(static_cast<const T*>(p.src[which]) + b * st.b + h * st.h + (i0 + i) * st.t + e0 * st.d, st.d,
+            p.vec[which] != 0, x);
+    }
+    const int64_t at = base + slot0 + i;
+    if constexpr (kInt8) {
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
+      for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // Scales stay at or above 2^-90, so that their inverses sum up in float32 (see fpa_decode_mma.cu); a row of
+      // zeros takes that smallest scale, so that it does not outweigh small rows there.
+      top = fmaxf(top, 127.f * 0x1p-90f);
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int code = min(max(__float2int_rn(__fdiv_rn(__fmul_rn(x[j], 127.f), top)), -127), 127);
+        w[j >> 2] |= uint32_t(code & 0xff) << (8 * (j & 3));
+      }
+      if (ok) {
+        char* dst = const_cast<char*>(static_cast<const char*>(which ? c.v : c.k)) + at * c.D + e0;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+        if (e0 == 0) const_cast<float*>(which ? c.vs : c.ks)[at] = __fdiv_rn(top, 127.f);
+      }
+    } else if (ok) {
+      store8(const_cast<T*>(static_cast<const T*>(which ? c.v : c.k)) + at * c.D + e0, x);
+    }
+  }
+  // The field, and the page's minimum over the slots up to the last one written.
+  float low = kInf;
+  float* phi = const_cast<float*>(c.phi) + base;
+  for (int s = threadIdx.x; s < slot0 + tokens; s += kThreads) {
+    float f;
+    if (s < slot0) {
+      f = phi[s];
+    } else {
+      const int i = i0 + s - slot0;
+      f = p.phi[b * p.sphi.b + h * p.sphi.h + i * p.sphi.t];
+      phi[s] = f;
+      const_cast<float*>(c.psi)[base + s] = p.psi[b * p.spsi.b + h * p.spsi.h + i * p.spsi.t];
+    }
+    low = fminf(low, f);
+  }
+  __shared__ float warp_low[kThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+  if ((threadIdx.x & 31) == 0) warp_low[threadIdx.x >> 5] = low;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kThreads / 32; ++w) low = fminf(low, warp_low[w]);
+    const_cast<float*>(c.pmin)[int64_t(pid) * c.H + h] = low;
+  }
+}
+
+struct ReadParams {
+  CacheView c;
+  const int32_t* table;
+  int64_t table_stride;
+  int max_pages, n;
+  const int32_t* start;
+  const int32_t* lengths;
+  void* k;
+  void* v;
+  float* phi;
+  float* psi;
+};
+
+// A block reads a run of kReadRows tokens of one (sequence, head).
+constexpr int kReadRows = 64;
+
+template <typename T, bool kInt8>
+__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const CacheView& c = p.c;
+  const int h = blockIdx.y, b = blockIdx.z, page = 1 << c.page_shift;
+  const int i0 = blockIdx.x * kReadRows, i1 = min(i0 + kReadRows, p.n);
+  const int64_t start = p.start ? p.start[b] : 0;
+  const int64_t cap = int64_t(p.max_pages) << c.page_shift;
+  const int64_t len = p.lengths ? min(int64_t(p.lengths[b]), cap) : cap;
+  if (threadIdx.x == 0 && blockIdx.x == 0 && (start < 0 || (p.lengths && p.lengths[b] > cap)))
+    report_bad_page(c.status, kSiteRead);
+  const int64_t out0 = (int64_t(b) * c.H + h) * p.n;
+  // Pool index of token i, or -1.
+  auto slot = [&](int i) -> int64_t {
+    const int64_t s = start + i;
+    if (s < 0 || s >= len) return -1;
+    const int pid = p.table[b * p.table_stride + (s >> c.page_shift)];
+    if (unsigned(pid) >= unsigned(c.n_pages)) {
+      report_bad_page(c.status, kSiteRead);
+      return -1;
+    }
+    return ((int64_t(pid) * c.H + h) << c.page_shift) + (s & (page - 1));
+  };
+  const int lanes = c.D >> 3, rows = kThreads / lanes;
+  const int sub = threadIdx.x / lanes, e0 = (threadIdx.x - sub * lanes) * 8;
+  for (int i = i0 + sub; i < i1; i += rows) {
+    const int64_t at = slot(i);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      if (at >= 0) {
+        const void* src = which ? c.v : c.k;
+        if constexpr (kInt8) {
+          const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const char*>(src) + at * c.D + e0);
+          const float scale = (which ? c.vs : c.ks)[at];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            x[j] = float(static_cast<signed char>((j < 4 ? w.x : w.y) >> (8 * (j & 3)))) * scale;
+        } else {
+          load8(static_cast<const T*>(src) + at * c.D + e0, 1, true, x);
+        }
+      }
+      store8(static_cast<T*>(which ? p.v : p.k) + (out0 + i) * c.D + e0, x);
+    }
+  }
+  for (int i = i0 + threadIdx.x; i < i1; i += kThreads) {
+    const int64_t at = slot(i);
+    p.phi[out0 + i] = at >= 0 ? c.phi[at] : 0.f;
+    p.psi[out0 + i] = at >= 0 ? c.psi[at] : 0.f;
+  }
+}
+
+int invalid(const char* msg) {
+  set_last_error(msg);
+  return FPA_ERR_INVALID_ARGUMENT;
+}
+
+int unsupported(const char* msg) {
+  set_last_error(msg);
+  return FPA_ERR_UNSUPPORTED;
+}
+
+int cuda_result(cudaError_t e, const char* where) {
+  if (e == cudaSuccess) return FPA_OK;
+  set_last_error(std::string(where) + ": " + cudaGetErrorString(e));
+  return FPA_ERR_CUDA;
+}
+
+// 16-byte reads of rows of eight elements: unit innermost stride, and everything else a multiple of 16 bytes.
+bool rows_aligned(const void* p, const int64_t st[4], int elem) {
+  if (reinterpret_cast<uintptr_t>(p) % 16 || st[3] != 1) return false;
+  for (int i = 0; i < 3; ++i)
+    if (st[i] * elem % 16) return false;
+  return true;
+}
+
+}  // namespace
+
+int check_cache(const FpaCache* c) {
+  if (c == nullptr) return invalid("null cache");
+  const bool f16 = c->dtype == FPA_DTYPE_F16;
+  if (!f16 && c->dtype != FPA_DTYPE_F32) return invalid("the cache's dtype must be fp16 or fp32");
+  if (c->storage != FPA_STORE_I8 && c->storage != (f16 ? FPA_STORE_F16 : FPA_STORE_F32))
+    return invalid("the cache's storage must be its dtype or int8");
+  if (c->n_pages <= 0 || c->H <= 0) return invalid("the cache needs at least one page and one head");
+  if (c->H > 65535) return unsupported("H above 65535 is not supported");
+  if (c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
+    return invalid("the page size must be 32, 64, 128 or 256");
+  if (c->D != 16 && c->D != 32 && c->D != 64 && c->D != 128 && c->D != 256)
+    return invalid("the head dimension must be 16, 32, 64, 128 or 256");
+  if (!c->k || !c->v || !c->phi || !c->psi || !c->phi_min || !c->status) return invalid("null cache pointer");
+  if (c->storage == FPA_STORE_I8 && (!c->k_scale || !c->v_scale)) return invalid("null cache scale pointer");
+  if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
+    return invalid("the cache's k and v must be 16-byte aligned");
+  return FPA_OK;
+}
+
+}  // namespace fpa
+
+using namespace fpa;
+
+extern "C" FPA_API int fpa_cache_append(const FpaAppendArgs* a, void* stream) {
+  if (a == nullptr) return invalid("null argument block");
+  if (const int rc = check_cache(a->cache)) return rc;
+  if (a->B <= 0 || a->n <= 0) return invalid("fpa_cache_append: B and n must be positive");
+  if (a->max_pages <= 0) return invalid("fpa_cache_append: the block table must have at least one column");
+  if (!a->k || !a->v || !a->phi || !a->psi || !a->table || !a->start) return invalid("fpa_cache_append: null tensor pointer");
+  if (a->B > 65535) return unsupported("fpa_cache_append: B above 65535 is not supported");
+  const FpaCache& c = *a->cache;
+  const int elem = c.dtype == FPA_DTYPE_F16 ? 2 : 4;
+  AppendParams p;
+  p.c = cache_view(c);
+  p.src[0] = a->k;
+  p.src[1] = a->v;
+  p.st[0] = str4(a->k_stride);
+  p.st[1] = str4(a->v_stride);
+  p.vec[0] = rows_aligned(a->k, a->k_stride, elem);
+  p.vec[1] = rows_aligned(a->v, a->v_stride, elem);
+  p.phi = a->phi;
+  p.psi = a->psi;
+  p.sphi = Str3{a->phi_stride[0], a->phi_stride[1], a->phi_stride[2]};
+  p.spsi = Str3{a->psi_stride[0], a->psi_stride[1], a->psi_stride[2]};
+  p.table = a->table;
+  p.table_stride = a->table_stride;
+  p.max_pages = a->max_pages;
+  p.n = a->n;
+  p.start = a->start;
+  p.counts = a->counts;
+  // n tokens touch at most this many pages, wherever they start.
+  const dim3 grid(unsigned((int64_t(a->n) + 2 * c.page_size - 2) / c.page_size), c.H, a->B);
+  const bool i8 = c.storage == FPA_STORE_I8;
+  auto kernel = c.dtype == FPA_DTYPE_F16 ? (i8 ? append_kernel<__half, true> : append_kernel<__half, false>)
+                                         : (i8 ? append_kernel<float, true> : append_kernel<float, false>);
+  return cuda_result(launch_pdl(kernel, grid, dim3(kThreads), 0, static_cast<cudaStream_t>(stream), p), "fpa_cache_append");
+}
+
+extern "C" FPA_API int fpa_cache_read(const FpaReadArgs* a, void* stream) {
+  if (a == nullptr) return invalid("null argument block");
+  if (const int rc = check_cache(a->cache)) return rc;
+  if (a->B <= 0 || a->n <= 0) return invalid("fpa_cache_read: B and n must be positive");
+  if (a->max_pages <= 0) return invalid("fpa_cache_read: the block table must have at least one column");
+  if (!a->k || !a->v || !a->phi || !a->psi || !a->table) return invalid("fpa_cache_read: null tensor pointer");
+  if (a->B > 65535) return unsupported("fpa_cache_read: B above 65535 is not supported");
+  if (reinterpret_cast<uintptr_t>(a->k) % 16 || reinterpret_cast<uintptr_t>(a->v) % 16)
+    return invalid("fpa_cache_read: k and v must be 16-byte aligned");
+  const FpaCache& c = *a->cache;
+  ReadParams p{cache_view(c), a->table, a->table_stride, a->max_pages, a->n, a->start, a->lengths, a->k, a->v, a->phi, a->psi};
+  const dim3 grid((unsigned(a->n) + kReadRows - 1) / kReadRows, c.H, a->B);
+  const bool i8 = c.storage == FPA_STORE_I8;
+  auto kernel = c.dtype == FPA_DTYPE_F16 ? (i8 ? read_kernel<__half, true> : read_kernel<__half, false>)
+                                         : (i8 ? read_kernel<float, true> : read_kernel<float, false>);
+  return cuda_result(launch_pdl(kernel, grid, dim3(kThreads), 0, static_cast<cudaStream_t>(stream), p), "fpa_cache_read");
+}

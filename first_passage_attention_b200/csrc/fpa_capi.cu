@@ -93,7 +93,17 @@ extern "C" {
 int fpa_abi_version(void) { return FPA_ABI_VERSION; }
 
 size_t fpa_struct_size(int which) {
-  return which == 0 ? sizeof(FpaFwdArgs) : which == 1 ? sizeof(FpaBwdArgs) : which == 2 ? sizeof(FpaFieldArgs) : 0;
+  switch (which) {
+    case 0: return sizeof(FpaFwdArgs);
+    case 1: return sizeof(FpaBwdArgs);
+    case 2: return sizeof(FpaFieldArgs);
+    case 3: return sizeof(FpaCache);
+    case 4: return sizeof(FpaAppendArgs);
+    case 5: return sizeof(FpaReadArgs);
+    case 6: return sizeof(FpaDecodeArgs);
+    case 7: return sizeof(FpaVerifyArgs);
+    default: return 0;
+  }
 }
 
 size_t fpa_fwd_workspace_bytes(int dtype, int B, int H, int T, int D, int path) {
@@ -223,7 +233,11 @@ int fpa_workspace_status(void* workspace, void* stream) {
   e = cudaMemcpyAsync(workspace, &zero, sizeof(int), cudaMemcpyHostToDevice, s);
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   char buf[128];
-  snprintf(buf, sizeof buf, "a bounded device-side wait expired (site %d)", v & 0xffff);
+  if ((v >> 16) == FPA_ERR_INVALID_ARGUMENT)
+    snprintf(buf, sizeof buf, "a length or position lies outside its block table, or a page id outside the cache (site %d)",
+             v & 0xffff);
+  else
+    snprintf(buf, sizeof buf, "a bounded device-side wait expired (site %d)", v & 0xffff);
   g_last_error = buf;
   return v >> 16;
 }

@@ -1,0 +1,306 @@
+// Attention of the newest tokens over the paged cache: the parts that the tensor-core and the FFMA kernels share.
+//
+// Row r of a sequence of L tokens stands at t = L - n + r and sees the keys s <= t with the logits
+//     z_ts = q_t k_s / sqrt(D) + beta min(0, min_{s<u<=t} phi_u - psi_s),   z_tt without the bias.
+// With Lb = L - n, the range minimum of a history key s < Lb splits into SUF_s = min_{s<u<Lb} phi_u, which all rows
+// share, and M_r = min_{Lb<=u<=t} phi_u, so the bias is beta min(a_s, M_r - psi_s) with a_s = min(0, SUF_s - psi_s);
+// the pairs among the n newest tokens get their minimum one by one. A prefix shared by the batch is the same thing once
+// more: its keys' SUF ends at the prefix's end and M_r is the minimum over the row's own tokens.
+//
+// What bounds it: the bytes of the cache. A CTA of four warps takes a (sequence, head, row group) or, as one of up to
+// 8 CTAs of a cluster, a part of its history; every warp walks its own consecutive run of 32-key tiles from the latest
+// to the earliest, so that SUF is a running minimum that the warp carries in a register, and no warp waits for
+// another until the end. What lies after a warp's run enters through the page minima (phi_min), four bytes a page and
+// head. The softmax states (m, l, O) of the warps join in shared memory, those of the cluster's CTAs through
+// distributed shared memory: one launch, no atomics, a fixed order.
+#pragma once
+
+#include "fpa_serve.h"
+
+namespace fpa {
+
+// The warp's minimum of phi over the positions [from, to) of a sequence: whole pages through phi_min, the rest from
+// phi itself.
+__device__ __forceinline__ float later_min(const CacheView& c, const int32_t* table, int h, int from, int to) {
+  const int lane = threadIdx.x & 31, page = 1 << c.page_shift;
+  float x = kInf;
+  const int e1 = min(to, (from + page - 1) & -page);
+  const int p1 = to >> c.page_shift;
+  const int e2 = max(e1, p1 << c.page_shift);
+  if (from < e1) {
+    const int pid = table[from >> c.page_shift];
+    if (unsigned(pid) < unsigned(c.n_pages)) {
+      const float* f = c.phi + ((int64_t(pid) * c.H + h) << c.page_shift);
+      for (int s = from + lane; s < e1; s += 32) x = fminf(x, f[s & (page - 1)]);
+    }
+  }
+  for (int pg = (e1 >> c.page_shift) + lane; pg < p1; pg += 32) {
+    const int pid = table[pg];
+    if (unsigned(pid) < unsigned(c.n_pages)) x = fminf(x, c.pmin[int64_t(pid) * c.H + h]);
+  }
+  if (e2 < to) {
+    const int pid = table[e2 >> c.page_shift];
+    if (unsigned(pid) < unsigned(c.n_pages)) {
+      const float* f = c.phi + ((int64_t(pid) * c.H + h) << c.page_shift);
+      for (int s = e2 + lane; s < to; s += 32) x = fminf(x, f[s & (page - 1)]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fminf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+// Index of slot `pos` of head h in the pool's [n_pages, H, page_size] arrays, or -1 where the table's entry lies
+// outside the pool (recorded in the status word).
+__device__ __forceinline__ int64_t slot_of(const CacheView& c, const int32_t* table, int h, int pos) {
+  const int pid = table[pos >> c.page_shift];
+  if (unsigned(pid) >= unsigned(c.n_pages)) {
+    report_bad_page(c.status, kSiteDecode);
+    return -1;
+  }
+  return ((int64_t(pid) * c.H + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+}
+
+// Minimum over the lanes' x of the lanes strictly after this one (+inf for lane 31); `all` gets the warp's minimum.
+__device__ __forceinline__ float suffix_min(float x, float& all) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float y = __shfl_down_sync(0xffffffffu, x, o);
+    if (lane + o < 32) x = fminf(x, y);
+  }
+  all = __shfl_sync(0xffffffffu, x, 0);
+  const float y = __shfl_down_sync(0xffffffffu, x, 1);
+  return lane < 31 ? y : kInf;
+}
+
+// Running minimum over the lanes up to and including this one.
+__device__ __forceinline__ float prefix_min(float x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x = fminf(x, y);
+  }
+  return x;
+}
+
+// The newest tokens of a sequence, one per lane (lanes >= nn hold nothing).
+struct NewTokens {
+  float phi, psi;  // +inf, 0 on the empty lanes
+  float low;       // min of phi over the new tokens up to this lane's
+  int64_t slot;    // pool index, or -1
+  int nn;
+};
+
+__device__ __forceinline__ NewTokens load_new(const CacheView& c, const int32_t* table, int h, int Lb, int nn) {
+  const int lane = threadIdx.x & 31;
+  NewTokens t{kInf, 0.f, kInf, -1, nn};
+  if (lane < nn) t.slot = slot_of(c, table, h, Lb + lane);
+  if (t.slot >= 0) {
+    t.phi = c.phi[t.slot];
+    t.psi = c.psi[t.slot];
+  }
+  t.low = prefix_min(t.phi);
+  return t;
+}
+
+// min_{j<u<=i} phi_u - psi_j, clamped at 0, for the new tokens j < i (0 for j == i). Warp-collective; j and i are the
+// calling lane's own.
+__device__ __forceinline__ float new_pair(const NewTokens& t, int j, int i) {
+  float m = kInf;
+  for (int u = 1; u < t.nn; ++u) {
+    const float f = __shfl_sync(0xffffffffu, t.phi, u);
+    if (u > j && u <= i) m = fminf(m, f);
+  }
+  const float psi = __shfl_sync(0xffffffffu, t.psi, j & 31);
+  return j < i ? fminf(m - psi, 0.f) : 0.f;
+}
+
+// What one CTA works on.
+struct Job {
+  const int32_t* table;
+  int h, b;
+  int rows;           // rows of this group
+  int r0;             // first row: of the sequence's n (decode) or of the head's R (prefix)
+  int end;            // history keys [0, end)
+  int t0, t1;         // this warp's tiles of 32 keys
+  int n_new;          // new tokens in the cache (decode)
+  int lead;           // rows of the sequence that stand before its first token
+  bool last;          // this warp also takes the tile of the new tokens
+  float bias;         // beta log2(e)
+};
+
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
+  uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(p)), r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float cluster_ld(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
+  return x;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// Weight of a softmax state with maximum m in a joint one with maximum M (0 for an empty state).
+__device__ __forceinline__ float state_weight(float m, float M) { return m == -kInf ? 0.f : ex2(m - M); }
+
+template <class Core>
+constexpr int decode_smem_floats() {
+  return ((Core::W * Core::NQ * (2 + Core::D) + 2 * Core::NQ + 3) & -4) + Core::kScratchFloats;
+}
+
+// Core: the arithmetic of one warp over a run of keys (see fpa_decode_mma.cu, fpa_decode_ffma.cu).
+// kPrefix: the rows (b, i) of the whole batch against the prefix, partial results to the workspace.
+template <class Core, bool kPrefix>
+__global__ void __launch_bounds__(Core::W * 32, Core::kMinBlocks) decode_kernel(const __grid_constant__ DecodeParams p) {
+  extern __shared__ __align__(16) float smem[];
+  constexpr int W = Core::W, NQ = Core::NQ, D = Core::D;
+  float* sO = smem;                 // [W][NQ][D]
+  float* sm = sO + W * NQ * D;      // [W][NQ]
+  float* sl = sm + W * NQ;          // [W][NQ]
+  float* cm = sl + W * NQ;          // [NQ]
+  float* cl = cm + NQ;              // [NQ]
+  float* scratch = smem + ((W * NQ * (2 + D) + 2 * NQ + 3) & -4);
+  const int warp = threadIdx.x >> 5;
+  const int S = gridDim.x, rank = blockIdx.x;
+  // A prefix pass before this kernel has waited for everything before it, so only its own results are still open:
+  // the wait then moves to where they are read.
+  const bool late = !kPrefix && p.prefix_len > 0;
+  if (!late) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
+  Job job;
+  int R = p.n;
+  if constexpr (kPrefix) {
+    job.h = blockIdx.z;
+    job.b = 0;
+    job.table = p.prefix_table;
+    job.end = p.prefix_len;
+    job.n_new = 0;
+    job.lead = 0;
+    job.r0 = blockIdx.y * NQ;
+    R = p.B * p.n;
+  } else {
+    job.h = blockIdx.y / p.groups;
+    job.r0 = (blockIdx.y - job.h * p.groups) * NQ;
+    job.b = blockIdx.z;
+    job.table = p.table + job.b * p.table_stride;
+    const int cap = int(min(int64_t(p.max_pages) << p.c.page_shift, int64_t(INT32_MAX)));
+    int L = p.lengths[job.b];
+    if (L < 0 || L > cap) {
+      report_bad_page(p.c.status, kSiteDecode);
+      L = min(max(L, 0), cap);
+    }
+    job.end = max(L - p.n, 0);
+    job.n_new = L - job.end;
+    job.lead = p.n - job.n_new;
+  }
+  job.rows = min(NQ, R - job.r0);
+  job.bias = p.beta[job.h] * kLog2e;
+  {
+    const int tiles = (job.end + 31) >> 5, units = S * W, u = rank * W + warp;
+    const int each = tiles / units, more = tiles - each * units;
+    job.t0 = u * each + min(u, more);
+    job.t1 = job.t0 + each + (u < more ? 1 : 0);
+    job.last = !kPrefix && u == units - 1;
+  }
+  Core core(p, job, scratch);
+  core.template run<kPrefix>(p, job);
+  core.store(sm + warp * NQ, sl + warp * NQ, sO + warp * NQ * D, job.rows);
+  __syncthreads();
+  // The CTA's state: maxima and sums per row, O in the first warp's place.
+  if (int(threadIdx.x) < job.rows) {
+    float M = -kInf, l = 0.f;
+    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w * NQ + threadIdx.x]);
+    for (int w = 0; w < W; ++w) l += sl[w * NQ + threadIdx.x] * state_weight(sm[w * NQ + threadIdx.x], M);
+    cm[threadIdx.x] = M;
+    cl[threadIdx.x] = l;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < job.rows * D; e += W * 32) {
+    const int r = e / D;
+    const float M = cm[r];
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) o += sO[w * NQ * D + e] * state_weight(sm[w * NQ + r], M);
+    if constexpr (kPrefix) {
+      const int64_t at = (int64_t(job.h) * R + job.r0 + r) * p.chunks + rank;
+      p.part_o[at * D + (e - r * D)] = o;
+      if (e == r * D) {
+        p.part_ml[at * 2] = M;
+        p.part_ml[at * 2 + 1] = cl[r];
+      }
+    } else {
+      sO[e] = o;
+    }
+  }
+  if constexpr (!kPrefix) {
+    if (late) pdl_wait();
+    if (S > 1)
+      cluster_barrier();
+    else
+      __syncthreads();
+    using O = typename Core::Out;
+    O* out = static_cast<O*>(p.o) + job.b * p.so.b + job.h * p.so.h;
+    for (int e = rank * W * 32 + threadIdx.x; e < job.rows * D; e += S * W * 32) {
+      const int r = e / D, d = e - r * D, row = job.r0 + r;
+      float M = -kInf;
+      const int64_t pre = ((int64_t(job.h) * p.B + job.b) * p.n + row) * p.chunks;
+      for (int c = 0; c < S; ++c) M = fmaxf(M, S > 1 ? cluster_ld(cluster_addr(cm + r, c)) : cm[r]);
+      if (late)
+        for (int c = 0; c < p.chunks; ++c) M = fmaxf(M, p.part_ml[(pre + c) * 2]);
+      float l = 0.f, o = 0.f;
+      for (int c = 0; c < S; ++c) {
+        const float w = state_weight(S > 1 ? cluster_ld(cluster_addr(cm + r, c)) : cm[r], M);
+        l += w * (S > 1 ? cluster_ld(cluster_addr(cl + r, c)) : cl[r]);
+        o += w * (S > 1 ? cluster_ld(cluster_addr(sO + e, c)) : sO[e]);
+      }
+      if (late)
+        for (int c = 0; c < p.chunks; ++c) {
+          const float w = state_weight(p.part_ml[(pre + c) * 2], M);
+          l += w * p.part_ml[(pre + c) * 2 + 1];
+          o += w * p.part_o[(pre + c) * D + d];
+        }
+      // Rows before the sequence's first token see nothing.
+      out[row * p.so.t + d * p.so.d] = from_f32<O>(row < job.lead ? 0.f : o / l);
+    }
+    if (S > 1) cluster_barrier();  // the other CTAs have read this one's shared memory
+  }
+}
+
+// Grid and launch of one pass. splits: CTAs of a cluster (own tokens) or parts of the prefix.
+template <class Core>
+cudaError_t launch_decode_core(DecodeParams p, bool prefix, int splits, cudaStream_t s) {
+  constexpr int smem = decode_smem_floats<Core>() * 4;
+  const int rows = prefix ? p.B * p.n : p.n;
+  p.groups = (rows + Core::NQ - 1) / Core::NQ;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = prefix ? dim3(splits, p.groups, p.c.H) : dim3(splits, p.c.H * p.groups, p.B);
+  cfg.blockDim = dim3(Core::W * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (!prefix && splits > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = splits;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  auto kernel = prefix ? decode_kernel<Core, true> : decode_kernel<Core, false>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+}  // namespace fpa

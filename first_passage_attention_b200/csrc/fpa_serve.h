@@ -1,0 +1,71 @@
+// Shared by the serving kernels (cache append / read, decode, verification): device views and host-side launchers.
+#pragma once
+
+#include "fpa_internal.h"
+
+namespace fpa {
+
+constexpr int kMaxNew = 16;  // newest tokens of one decode call
+
+// Sites that the cache's status word names next to FPA_ERR_INVALID_ARGUMENT.
+enum ServeSite { kSiteAppend = 1, kSiteRead = 2, kSiteDecode = 3 };
+
+struct CacheView {
+  const void* k;
+  const void* v;
+  const float* ks;
+  const float* vs;
+  const float* phi;
+  const float* psi;
+  const float* pmin;
+  int* status;
+  int n_pages, H, page_shift, D;
+};
+
+inline int log2_int(int x) {
+  int n = 0;
+  while ((1 << n) < x) ++n;
+  return n;
+}
+
+inline CacheView cache_view(const FpaCache& c) {
+  return CacheView{c.k, c.v, c.k_scale, c.v_scale, c.phi, c.psi, c.phi_min, c.status, c.n_pages, c.H,
+                   log2_int(c.page_size), c.D};
+}
+
+__device__ __forceinline__ void report_bad_page(int* status, int site) {
+  if (status) atomicCAS(status, 0, (FPA_ERR_INVALID_ARGUMENT << 16) | site);
+}
+
+struct DecodeParams {
+  CacheView c;
+  const void* q;
+  Str4 sq;
+  void* o;
+  Str4 so;
+  const float* beta;
+  const int32_t* table;
+  int64_t table_stride;
+  int max_pages;
+  const int32_t* lengths;
+  const int32_t* prefix_table;
+  int prefix_pages, prefix_len;
+  int B, n;
+  int groups;      // row groups of a (sequence, head) (decode) or of a head (prefix pass)
+  int q_pairs;     // q can be read two elements at a time
+  float scale2;    // log2(e) / sqrt(D)
+  // Prefix: rows are (b, i) in b-major order, R = B * n of them for each head.
+  float* row_min;  // [H][R]  minimum of phi over the row's own tokens up to itself
+  float* part_ml;  // [H][R][chunks][2]  softmax maximum and sum of each chunk of the prefix
+  float* part_o;   // [H][R][chunks][D]  unnormalised output of each chunk
+  int chunks;
+};
+
+// Rows are handled by one CTA in groups of 8 or 16 (tensor cores) or 1, 4 or 8 (FFMA).
+cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, int splits, cudaStream_t s);
+cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, int splits, cudaStream_t s);
+cudaError_t launch_row_min(const DecodeParams& p, cudaStream_t s);
+
+int sm_count();  // fpa_tma.cu
+
+}  // namespace fpa

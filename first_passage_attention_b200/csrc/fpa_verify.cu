@@ -1,0 +1,175 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// Draft i is accepted while u_i q_i(x_i) < p_i(x_i). With a drafts accepted, the next token is a sample of the
+// normalised residual max(p_a - q_a, 0) (of p_a when all drafts were accepted, or when the residual vanishes): for noise
+// e_v from the exponential distribution, argmax_v w_v / e_v has the distribution w / sum w, so the weights need no
+// sum, and each score is one subtraction and one division, rounded once each: the token does not depend on how the
+// vocabulary is cut up.
+//
+// Bound by the bytes of three rows of V per sequence. A cluster of CTAs shares a sequence; every CTA finds `a` itself
+// (a few gathers), takes a part of the vocabulary and leaves its best (score, index) in shared memory, which the first
+// CTA compares through distributed shared memory.
+#include "fpa_serve.h"
+
+namespace fpa {
+namespace {
+
+constexpr int kThreads = 512;
+
+struct VerifyParams {
+  const void* p;
+  const void* q;
+  int64_t pb, pt, qb, qt;
+  const int64_t* draft;
+  int64_t db, dt;
+  const float* u;
+  int64_t ub, ut;
+  const float* noise;
+  int64_t nb;
+  const int32_t* lens;
+  int32_t* accepted;
+  int64_t* tokens;
+  int n, V;
+};
+
+// Scores are >= 0, so their bits order as they do; the complement of the index lets the lowest index win a tie.
+__device__ __forceinline__ unsigned long long key_of(float w, float e, int v) {
+  const float score = __fdiv_rn(w, e);
+  if (!(w > 0.f) || !(score >= 0.f)) return 0ull;
+  return (static_cast<unsigned long long>(__float_as_uint(score) + 1u) << 32) | (0xffffffffu - unsigned(v));
+}
+
+// Best key of the block (in every thread of warp 0); `red` holds one key per warp.
+__device__ __forceinline__ unsigned long long block_best(unsigned long long k, unsigned long long* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = k;
+  __syncthreads();
+  k = (threadIdx.x & 31) < kThreads / 32 ? red[threadIdx.x & 31] : 0ull;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+  __syncthreads();
+  return k;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ VerifyParams a) {
+  __shared__ unsigned long long red[kThreads / 32], best[2];
+  __shared__ int first;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int S = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
+  const T* P = static_cast<const T*>(a.p) + b * a.pb;
+  const T* Q = static_cast<const T*>(a.q) + b * a.qb;
+  const int n = a.lens ? min(max(a.lens[b], 0), a.n) : a.n;
+  if (threadIdx.x < 32) {
+    // The first refused draft: 32 at a time.
+    int acc = n;
+    for (int i0 = 0; i0 < n && acc == n; i0 += 32) {
+      const int i = i0 + int(threadIdx.x);
+      bool refuse = false;
+      if (i < n) {
+        const int64_t x = a.draft[b * a.db + i * a.dt];
+        refuse = x < 0 || x >= a.V ||
+                 !(__fmul_rn(a.u[b * a.ub + i * a.ut], to_f32(Q[i * a.qt + x])) < to_f32(P[i * a.pt + x]));
+      }
+      const unsigned m = __ballot_sync(0xffffffffu, refuse);
+      if (m) acc = i0 + __ffs(m) - 1;
+    }
+    if (threadIdx.x == 0) first = acc;
+  }
+  __syncthreads();
+  const int acc = first;
+  const T* pr = P + acc * a.pt;
+  const T* qr = acc < n ? Q + acc * a.qt : nullptr;
+  const float* e = a.noise + b * a.nb;
+  // The residual's best and, for a residual of nothing, the target's own best.
+  unsigned long long kr = 0, kp = 0;
+  for (int v = rank * kThreads + int(threadIdx.x); v < a.V; v += S * kThreads) {
+    const float pv = to_f32(pr[v]), ev = e[v];
+    if (qr) {
+      kr = max(kr, key_of(__fsub_rn(pv, to_f32(qr[v])), ev, v));
+    }
+    kp = max(kp, key_of(pv, ev, v));
+  }
+  kr = block_best(kr, red);
+  kp = block_best(kp, red);
+  if (threadIdx.x == 0) {
+    best[0] = kr;
+    best[1] = kp;
+  }
+  if (S > 1) {
+    cluster_sync();
+    if (rank == 0 && threadIdx.x == 0) {
+      for (int c = 1; c < S; ++c) {
+        uint32_t at;
+        unsigned long long x, y;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(best))), "r"(c));
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(at) : "memory");
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(y) : "r"(at + 8) : "memory");
+        kr = max(kr, x);
+        kp = max(kp, y);
+      }
+    }
+    cluster_sync();
+  }
+  if (rank == 0 && threadIdx.x < 32) {
+    const unsigned long long k = __shfl_sync(0xffffffffu, kr ? kr : kp, 0);
+    // Nothing positive anywhere (all zeros or NaN): the lowest index.
+    const int64_t next = k ? int64_t(0xffffffffu - unsigned(k)) : 0;
+    for (int i = threadIdx.x; i <= a.n; i += 32)
+      a.tokens[int64_t(b) * (a.n + 1) + i] = i < acc ? a.draft[b * a.db + i * a.dt] : i == acc ? next : -1;
+    if (threadIdx.x == 0) a.accepted[b] = acc;
+  }
+}
+
+int invalid(const char* msg) {
+  set_last_error(msg);
+  return FPA_ERR_INVALID_ARGUMENT;
+}
+
+}  // namespace
+}  // namespace fpa
+
+using namespace fpa;
+
+extern "C" FPA_API int fpa_verify(const FpaVerifyArgs* a, void* stream) {
+  if (a == nullptr) return invalid("null argument block");
+  if (a->dtype != FPA_DTYPE_F16 && a->dtype != FPA_DTYPE_F32) return invalid("fpa_verify: p and q must be fp16 or fp32");
+  if (a->B <= 0 || a->n < 0 || a->V <= 0) return invalid("fpa_verify: B and V must be positive and n not negative");
+  if (!a->p || !a->noise || !a->accepted || !a->tokens || (a->n > 0 && (!a->q || !a->draft || !a->u)))
+    return invalid("fpa_verify: null tensor pointer");
+  if (a->B > 65535) {
+    set_last_error("fpa_verify: B above 65535 is not supported");
+    return FPA_ERR_UNSUPPORTED;
+  }
+  VerifyParams p{a->p, a->q, a->p_stride[0], a->p_stride[1], a->q_stride[0], a->q_stride[1], a->draft, a->draft_stride[0],
+                 a->draft_stride[1], a->u, a->u_stride[0], a->u_stride[1], a->noise, a->noise_stride, a->draft_lens,
+                 a->accepted, a->tokens, a->n, a->V};
+  // Up to 8 CTAs for a sequence, while the grid leaves SMs idle and every thread keeps an entry.
+  int S = 1;
+  while (S < 8 && a->B * S < 2 * sm_count() && S * kThreads < a->V) S *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(S, a->B);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = S;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = S > 1 ? 2 : 1;
+  const cudaError_t e = a->dtype == FPA_DTYPE_F16 ? cudaLaunchKernelEx(&cfg, verify_kernel<__half>, p)
+                                                  : cudaLaunchKernelEx(&cfg, verify_kernel<float>, p);
+  if (e != cudaSuccess) {
+    set_last_error(std::string("fpa_verify: ") + cudaGetErrorString(e));
+    return FPA_ERR_CUDA;
+  }
+  return FPA_OK;
+}

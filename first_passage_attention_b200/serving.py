@@ -1,0 +1,238 @@
+"""Serving a model with First Passage Attention: the paged cache, attention of the newest tokens over it, and the
+verification of drafted tokens. Forward only; every call runs the native kernels of libfpa_b200 on the current stream,
+allocates its outputs only, never synchronises, and can be captured in a CUDA graph.
+
+``FPACache`` holds keys, values and the field of many sequences in pages of a common pool, as the model's fp16 or fp32
+values or as int8 codes with a scale for each token and head. A sequence's position s lies in page
+``block_table[b, s // page_size]``; block tables, lengths and start positions are int32 tensors on the device.
+
+    cache = FPACache(n_pages, n_heads, head_dim, dtype=torch.float16, storage=torch.int8)
+    cache.append(k, v, phi, psi, block_table, start)                    # k, v [B, H, n, D], phi, psi [B, H, n]
+    o = first_passage_decode(q, cache, block_table, start + n, beta)    # q, o [B, H, n, D], n from 1 to 16
+
+The walk of the field is cumulative, so phi and psi of new tokens go on from the walk's last value; the model keeps it
+(``LMGenerator`` in ``lm.py`` does).
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from .ops import LaunchStats, _on_device, _stream
+
+MAX_NEW_TOKENS = 16
+_PAGE_SIZES = (32, 64, 128, 256)
+_HEAD_DIMS = (16, 32, 64, 128, 256)
+
+
+def _int32_on(name, x, device, shape=None):
+    if x.dtype != torch.int32 or x.device != device:
+        raise ValueError(f"{name} must be an int32 tensor on {device}")
+    if shape is not None and (x.shape != shape or not x.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous with shape {tuple(shape)}")
+    return x.data_ptr()
+
+
+def _table_on(name, x, device, B):
+    if x.dtype != torch.int32 or x.device != device:
+        raise ValueError(f"{name} must be an int32 tensor on {device}")
+    if x.dim() != 2 or x.shape[0] != B or x.shape[1] < 1 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError(f"{name} must have shape (B, pages) with contiguous rows")
+    return x.data_ptr(), x.stride(0), x.shape[1]
+
+
+def _call(fn, args, device):
+    with _on_device(device):
+        _lib.check(fn(ctypes.byref(args), _stream(device)))
+
+
+class FPACache:
+    """A pool of pages of keys, values and the field, for every head: k and v [n_pages, n_heads, page_size, head_dim],
+    phi and psi [n_pages, n_heads, page_size]; with ``storage=torch.int8`` also k_scale and v_scale of phi's shape.
+    phi_min [n_pages, n_heads] is the minimum of phi over each page (``append`` maintains it; decoding relies on it
+    for pages that a sequence has filled).
+
+    dtype: of k, v, q and o (float16 or float32). storage: None (as dtype) or torch.int8: scale = max|x| / 127 for each
+    token and head, code = round(127 x / max|x|), the value is code * scale."""
+
+    def __init__(self, n_pages, n_heads, head_dim, page_size=64, dtype=torch.float16, storage=None, device="cuda"):
+        if dtype not in (torch.float16, torch.float32):
+            raise ValueError("the cache's dtype must be float16 or float32")
+        if storage not in (None, dtype, torch.int8):
+            raise ValueError("the cache's storage must be its dtype or int8")
+        if page_size not in _PAGE_SIZES:
+            raise ValueError("the page size must be 32, 64, 128 or 256")
+        if head_dim not in _HEAD_DIMS:
+            raise ValueError("the head dimension must be 16, 32, 64, 128 or 256")
+        if n_pages < 1 or n_heads < 1:
+            raise ValueError("the cache needs at least one page and one head")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("the cache needs a CUDA device")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.n_pages, self.n_heads, self.head_dim, self.page_size = n_pages, n_heads, head_dim, page_size
+        self.dtype, self.storage, self.device = dtype, storage or dtype, device
+        slots = (n_pages, n_heads, page_size)
+        self.k = torch.zeros(*slots, head_dim, dtype=self.storage, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.phi, self.psi = torch.zeros(slots, device=device), torch.zeros(slots, device=device)
+        self.phi_min = torch.zeros(slots[:2], device=device)
+        self.k_scale = self.v_scale = None
+        if self.storage == torch.int8:
+            self.k_scale, self.v_scale = torch.zeros(slots, device=device), torch.zeros(slots, device=device)
+        self._status = torch.zeros(64, dtype=torch.int32, device=device)
+        self._struct = _lib.FpaCache(
+            _lib.DTYPE_F16 if dtype == torch.float16 else _lib.DTYPE_F32,
+            {torch.float16: _lib.STORE_F16, torch.float32: _lib.STORE_F32, torch.int8: _lib.STORE_I8}[self.storage],
+            n_pages, n_heads, page_size, head_dim,
+            *(None if x is None else x.data_ptr() for x in (self.k, self.v, self.k_scale, self.v_scale, self.phi,
+                                                            self.psi, self.phi_min, self._status)))
+        self._addr = ctypes.addressof(self._struct)
+
+    def append(self, k, v, phi, psi, block_table, start, counts=None):
+        """Write the tokens k, v [B, H, n, D], phi, psi [B, H, n] (any strides) at positions start[b], start[b] + 1, ...
+        of each sequence: counts[b] of them, or all n. They become the sequence's newest tokens: whatever it held from
+        there on is gone (that is also how refused drafts are taken back)."""
+        lib = _lib.load()
+        H, D = self.n_heads, self.head_dim
+        if k.dim() != 4 or v.shape != k.shape or k.shape[1] != H or k.shape[3] != D:
+            raise ValueError(f"k and v must have shape (B, {H}, n, {D})")
+        if k.dtype != self.dtype or v.dtype != self.dtype:
+            raise ValueError(f"k and v must be {self.dtype}")
+        B, _, n, _ = k.shape
+        if phi.shape != k.shape[:3] or psi.shape != phi.shape:
+            raise ValueError(f"phi and psi must have shape (B, {H}, n)")
+        if phi.dtype != torch.float32 or psi.dtype != torch.float32:
+            raise ValueError("phi and psi must be float32")
+        dev = self.device
+        if k.device != dev or v.device != dev or phi.device != dev or psi.device != dev:
+            raise ValueError(f"k, v, phi and psi must be on the cache's device {dev}")
+        if B == 0 or n == 0:
+            return
+        a = _lib.FpaAppendArgs()
+        _lib.APPEND_PACKER.pack_into(
+            a, 0, self._addr, B, n, k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), phi.data_ptr(), *phi.stride(),
+            psi.data_ptr(), *psi.stride(), *_table_on("block_table", block_table, dev, B),
+            _int32_on("start", start, dev, (B,)), 0 if counts is None else _int32_on("counts", counts, dev, (B,)))
+        _call(lib.fpa_cache_append, a, dev)
+        LaunchStats.kernels += 1
+
+    def read(self, block_table, start, n, lengths=None):
+        """k, v [B, H, n, D] in the cache's dtype and phi, psi [B, H, n] at positions start[b] .. start[b] + n - 1 (from
+        0 with start None); positions from lengths[b] on (or beyond the table) are zeros."""
+        lib = _lib.load()
+        B, H, D, dev = block_table.shape[0], self.n_heads, self.head_dim, self.device
+        if n < 0:
+            raise ValueError("n must not be negative")
+        table = _table_on("block_table", block_table, dev, B)
+        start = 0 if start is None else _int32_on("start", start, dev, (B,))
+        lengths = 0 if lengths is None else _int32_on("lengths", lengths, dev, (B,))
+        k = torch.empty((B, H, n, D), dtype=self.dtype, device=dev)
+        v = torch.empty_like(k)
+        phi = torch.empty((B, H, n), dtype=torch.float32, device=dev)
+        psi = torch.empty_like(phi)
+        if B and n:
+            a = _lib.FpaReadArgs()
+            _lib.READ_PACKER.pack_into(a, 0, self._addr, B, n, *table, start, lengths, k.data_ptr(), v.data_ptr(),
+                                       phi.data_ptr(), psi.data_ptr())
+            _call(lib.fpa_cache_read, a, dev)
+            LaunchStats.kernels += 1
+        return k, v, phi, psi
+
+    def check(self):
+        """Synchronise, and raise if a call since the last check met a page id outside the pool, or a position or
+        length outside a block table (such entries are skipped, never touched)."""
+        lib = _lib.load()
+        with _on_device(self.device):
+            _lib.check(lib.fpa_workspace_status(ctypes.c_void_p(self._status.data_ptr()), _stream(self.device)))
+
+
+def first_passage_decode(q, cache, block_table, lengths, beta, prefix_table=None, prefix_len=0):
+    """o [B, H, n, D] of the newest n tokens (1 to 16) of each sequence, which ``cache.append`` has stored already.
+
+    q: [B, H, n, D] in the cache's dtype (any strides). lengths[b] counts the sequence's tokens, the new ones included;
+    row r stands at position lengths[b] - n + r, and rows before position 0 come out as zeros (length 0: an idle slot).
+    beta: [H] float32. prefix_table (int32, [pages]) and prefix_len: tokens in the cache that come before the first
+    token of every sequence, such as a system prompt; lengths do not count them, and they are read once for the whole
+    batch. Equal to the last n rows of ``first_passage_attention`` over the whole sequence."""
+    lib = _lib.load()
+    H, D, dev = cache.n_heads, cache.head_dim, cache.device
+    if q.dim() != 4 or q.shape[1] != H or q.shape[3] != D:
+        raise ValueError(f"q must have shape (B, {H}, n, {D})")
+    B, _, n, _ = q.shape
+    if not 1 <= n <= MAX_NEW_TOKENS:
+        raise ValueError(f"between 1 and {MAX_NEW_TOKENS} new tokens per call")
+    if q.dtype != cache.dtype or q.device != dev:
+        raise ValueError(f"q must be {cache.dtype} on {dev}")
+    if beta.shape != (H,) or beta.dtype != torch.float32 or beta.device != dev or not beta.is_contiguous():
+        raise ValueError(f"beta must be a contiguous float32 tensor of shape ({H},) on {dev}")
+    pages, ptable = 0, 0
+    if prefix_len < 0 or (prefix_len > 0 and prefix_table is None):
+        raise ValueError("prefix_len must not be negative, and needs a prefix_table")
+    if prefix_len > 0:
+        pages = prefix_table.numel()
+        ptable = _int32_on("prefix_table", prefix_table, dev, (pages,))
+        if pages * cache.page_size < prefix_len:
+            raise ValueError("the prefix is longer than the pages of its table")
+    o = torch.empty((B, H, n, D), dtype=q.dtype, device=dev)
+    if B == 0:
+        return o
+    table = _table_on("block_table", block_table, dev, B)
+    lengths = _int32_on("lengths", lengths, dev, (B,))
+    ws, ws_ptr, nbytes = None, 0, 0
+    with _on_device(dev):
+        if prefix_len > 0:
+            nbytes = lib.fpa_decode_workspace_bytes(ctypes.byref(cache._struct), B, n, prefix_len)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ws_ptr = ws.data_ptr()
+        a = _lib.FpaDecodeArgs()
+        _lib.DECODE_PACKER.pack_into(a, 0, cache._addr, B, n, q.data_ptr(), *q.stride(), o.data_ptr(), *o.stride(),
+                                     beta.data_ptr(), *table, lengths, ptable, pages, prefix_len, ws_ptr, nbytes, 0)
+        _lib.check(lib.fpa_decode(ctypes.byref(a), _stream(dev)))
+    LaunchStats.kernels += a.kernels_launched
+    return o
+
+
+def verify_draft(p, q, draft, u, noise, draft_lens=None):
+    """Accept drafted tokens against the target's probabilities, from given random numbers.
+
+    p [B, n + 1, V]: the target's probabilities after 0, 1, ... n drafted tokens; q [B, n, V]: those that the drafts were
+    drawn from (both fp16 or both fp32); draft [B, n] int64; u [B, n] float32 from [0, 1); noise [B, V] float32 from the
+    exponential distribution; draft_lens [B] int32: drafts of each sequence where they are fewer than n.
+
+    Draft i is accepted while u_i q_i(x_i) < p_i(x_i). Returns accepted [B] int32 (drafts before the first refusal) and
+    tokens [B, n + 1] int64: the accepted drafts, the next token, then -1. The next token is argmax_v max(p_a - q_a, 0) /
+    noise (a draw from the normalised residual), or argmax_v p_a / noise where every draft was accepted or the residual
+    is nowhere positive; ties go to the lowest index. The tokens then have the target's distribution."""
+    lib = _lib.load()
+    if p.dim() != 3 or q.dim() != 3 or q.shape[0] != p.shape[0] or q.shape[2] != p.shape[2] or p.shape[1] != q.shape[1] + 1:
+        raise ValueError("p must have shape (B, n + 1, V) and q shape (B, n, V)")
+    B, n, V = q.shape
+    if p.dtype not in (torch.float16, torch.float32) or q.dtype != p.dtype:
+        raise ValueError("p and q must both be fp16 or both fp32")
+    if draft.shape != (B, n) or draft.dtype != torch.int64:
+        raise ValueError("draft must be an int64 tensor of shape (B, n)")
+    if u.shape != (B, n) or u.dtype != torch.float32:
+        raise ValueError("u must be a float32 tensor of shape (B, n)")
+    if noise.shape != (B, V) or noise.dtype != torch.float32:
+        raise ValueError("noise must be a float32 tensor of shape (B, V)")
+    if V < 1:
+        raise ValueError("the vocabulary must not be empty")
+    dev = p.device
+    if not p.is_cuda or any(x.device != dev for x in (q, draft, u, noise)):
+        raise ValueError("p, q, draft, u and noise must be on one CUDA device")
+    p, q, noise = (x if x.stride(-1) == 1 else x.contiguous() for x in (p, q, noise))
+    lens = 0 if draft_lens is None else _int32_on("draft_lens", draft_lens, dev, (B,))
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    tokens = torch.empty((B, n + 1), dtype=torch.int64, device=dev)
+    if B == 0:
+        return accepted, tokens
+    a = _lib.FpaVerifyArgs()
+    _lib.VERIFY_PACKER.pack_into(
+        a, 0, _lib.DTYPE_F16 if p.dtype == torch.float16 else _lib.DTYPE_F32, B, n, V, p.data_ptr(), *p.stride()[:2],
+        q.data_ptr(), *q.stride()[:2], draft.data_ptr(), *draft.stride(), u.data_ptr(), *u.stride(), noise.data_ptr(),
+        noise.stride(0), lens, accepted.data_ptr(), tokens.data_ptr())
+    _call(lib.fpa_verify, a, dev)
+    LaunchStats.kernels += 1
+    return accepted, tokens

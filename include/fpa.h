@@ -117,11 +117,102 @@ typedef struct FpaFieldArgs {
   float* dproj; int64_t dproj_stride[3]; /* out (backward) */
 } FpaFieldArgs;
 
+/* ---------------------------------------------------------------------------------------------- serving ----------
+ * A paged cache of keys, values and the field (phi, psi), attention of the newest tokens over it, and the verification
+ * of drafted tokens. No counterpart in the reference (which trains only). Forward only.
+ *
+ * The pool holds n_pages pages of page_size tokens for every head. A sequence owns a row of a block table: its
+ * position s lies in page table[s / page_size], slot s % page_size. Page ids outside [0, n_pages), positions beyond
+ * the table's row and negative positions are never touched: the call skips them and records
+ * FPA_ERR_INVALID_ARGUMENT in the cache's status word (read it with fpa_workspace_status). */
+enum FpaStorage { FPA_STORE_F16 = 0, FPA_STORE_F32 = 1, FPA_STORE_I8 = 2 };
+
+typedef struct FpaCache {
+  int32_t dtype;            /* FpaDtype of k, v as handed in and out, and of q and o */
+  int32_t storage;          /* FpaStorage: that type, or int8 codes with a float32 scale per token and head */
+  int32_t n_pages, H;
+  int32_t page_size;        /* 32, 64, 128 or 256 */
+  int32_t D;                /* 16, 32, 64, 128 or 256 */
+  void* k;                  /* [n_pages, H, page_size, D], 16-byte aligned */
+  void* v;                  /* [n_pages, H, page_size, D], 16-byte aligned */
+  float* k_scale;           /* [n_pages, H, page_size] (int8 storage; else ignored) */
+  float* v_scale;
+  float* phi;               /* [n_pages, H, page_size] */
+  float* psi;
+  float* phi_min;           /* [n_pages, H]: minimum of phi over the page, valid once the page is full */
+  int32_t* status;          /* one word, zero before the first call */
+} FpaCache;
+
+/* Appends counts[b] tokens (all n if counts is null) to each sequence at its positions start[b], start[b] + 1, ...
+ * Later positions of the sequence are no longer part of it. int8: scale = max|x| / 127 (at least 2^-90), code =
+ * rint(127 x / max|x|), the value is code * scale. phi_min of the touched pages is brought up to date. */
+typedef struct FpaAppendArgs {
+  const FpaCache* cache;
+  int32_t B, n;
+  const void* k; int64_t k_stride[4];       /* [B, H, n, D] in the cache's dtype, any strides */
+  const void* v; int64_t v_stride[4];
+  const float* phi; int64_t phi_stride[3];  /* [B, H, n] */
+  const float* psi; int64_t psi_stride[3];
+  const int32_t* table; int64_t table_stride; int32_t max_pages; /* [B, max_pages] */
+  const int32_t* start;                     /* [B] */
+  const int32_t* counts;                    /* [B] or null */
+} FpaAppendArgs;
+
+/* Reads positions start[b] .. start[b] + n - 1 (start null: from 0) into dense tensors; positions at or beyond
+ * lengths[b] (null: all positions of the table's row) give zeros. */
+typedef struct FpaReadArgs {
+  const FpaCache* cache;
+  int32_t B, n;
+  const int32_t* table; int64_t table_stride; int32_t max_pages;
+  const int32_t* start;                     /* [B] or null */
+  const int32_t* lengths;                   /* [B] or null */
+  void* k; void* v;                         /* out: [B, H, n, D] contiguous in the cache's dtype, 16-byte aligned */
+  float* phi; float* psi;                   /* out: [B, H, n] contiguous */
+} FpaReadArgs;
+
+/* Attention of the newest n tokens of each sequence (1 <= n <= 16), which are in the cache already: lengths[b] counts
+ * them, and row r of sequence b stands at its position lengths[b] - n + r. Rows at negative positions come out as
+ * zeros (a sequence of length 0 is an idle slot). With a prefix (prefix_len > 0), the prefix's tokens, which lie in
+ * the pages of prefix_table, come before the first token of every sequence; lengths do not count them. */
+typedef struct FpaDecodeArgs {
+  const FpaCache* cache;
+  int32_t B, n;
+  const void* q; int64_t q_stride[4];       /* [B, H, n, D], any strides */
+  void* o; int64_t o_stride[4];             /* [B, H, n, D], any strides */
+  const float* beta;                        /* [H] */
+  const int32_t* table; int64_t table_stride; int32_t max_pages;
+  const int32_t* lengths;                   /* [B] */
+  const int32_t* prefix_table;              /* [prefix_pages] or null */
+  int32_t prefix_pages;
+  int32_t prefix_len;                       /* at most prefix_pages * page_size */
+  void* workspace;                          /* fpa_decode_workspace_bytes(...) bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  int32_t kernels_launched;                 /* out */
+} FpaDecodeArgs;
+
+/* Verification of n drafted tokens per sequence (draft_lens[b] <= n of them where given) against the target's
+ * probabilities. Draft i is accepted while u_i q_i(x_i) < p_i(x_i); a is the number accepted before the first refusal.
+ * The next token is argmax_v max(p_a(v) - q_a(v), 0) / noise(v) (p_a(v) / noise(v) where all drafts are accepted, or
+ * where p_a exceeds q_a nowhere); with noise from the exponential distribution that is a sample of the residual.
+ * Ties go to the lowest index. Products, differences and quotients are rounded once each, in float32. */
+typedef struct FpaVerifyArgs {
+  int32_t dtype;                            /* FpaDtype of p and q */
+  int32_t B, n, V;                          /* n >= 0, V >= 1 */
+  const void* p; int64_t p_stride[2];       /* [B, n + 1, V], rows contiguous */
+  const void* q; int64_t q_stride[2];       /* [B, n, V], rows contiguous */
+  const int64_t* draft; int64_t draft_stride[2]; /* [B, n], values in [0, V); others are refused */
+  const float* u; int64_t u_stride[2];      /* [B, n] */
+  const float* noise; int64_t noise_stride; /* [B, V], rows contiguous */
+  const int32_t* draft_lens;                /* [B] or null */
+  int32_t* accepted;                        /* out: [B] */
+  int64_t* tokens;                          /* out: [B, n + 1] contiguous: accepted drafts, the next token, then -1 */
+} FpaVerifyArgs;
+
 /* ABI version of the loaded library (FPA_ABI_VERSION). */
 FPA_API int fpa_abi_version(void);
 
-/* sizeof(FpaFwdArgs) for which == 0, sizeof(FpaBwdArgs) for 1, sizeof(FpaFieldArgs) for 2; lets bindings check their
- * struct mirrors. */
+/* sizeof(FpaFwdArgs) for which == 0, sizeof(FpaBwdArgs) for 1, sizeof(FpaFieldArgs) for 2, FpaCache 3, FpaAppendArgs 4,
+ * FpaReadArgs 5, FpaDecodeArgs 6, FpaVerifyArgs 7; lets bindings check their struct mirrors. */
 FPA_API size_t fpa_struct_size(int which);
 
 /* Workspace sizes in bytes for a call with these sizes (0 for invalid sizes). Call them with the device that will run
@@ -143,7 +234,9 @@ FPA_API int fpa_field_fwd(const FpaFieldArgs* args, void* stream);
 FPA_API int fpa_field_bwd(const FpaFieldArgs* args, void* stream);
 
 /* Synchronises `stream`, then reads and clears the device status word at the head of a workspace that a previous
- * fpa_fwd / fpa_bwd call used: FPA_OK, or FPA_ERR_TIMEOUT if a bounded device-side wait expired in that call. */
+ * fpa_fwd / fpa_bwd call used: FPA_OK, or FPA_ERR_TIMEOUT if a bounded device-side wait expired in that call. Also
+ * reads the status word of an FpaCache: FPA_ERR_INVALID_ARGUMENT if a call met a page id, position or length out of
+ * range. */
 FPA_API int fpa_workspace_status(void* workspace, void* stream);
 
 /* Human-readable text for an FpaStatus, or the message of the last argument error on this thread. */
@@ -186,6 +279,15 @@ FPA_API int fpa_selftest_wait_timeout(void* workspace, unsigned long long limit_
  * set-up call fpa_fwd_noalloc(NULL, stream), which launches nothing, and before any stream capture. All calls
  * share the one array: calls whose kernels overlap on the GPU race and must be serialised by the caller. */
 FPA_API int fpa_fwd_noalloc(FpaFwdArgs* args, void* stream);
+
+/* Serving (see FpaCache above): each call is asynchronous on `stream` and returns an FpaStatus. */
+FPA_API int fpa_cache_append(const FpaAppendArgs* args, void* stream);
+FPA_API int fpa_cache_read(const FpaReadArgs* args, void* stream);
+FPA_API int fpa_decode(FpaDecodeArgs* args, void* stream);
+FPA_API int fpa_verify(const FpaVerifyArgs* args, void* stream);
+
+/* Workspace of fpa_decode in bytes (0 without a prefix: none is needed), on the current device. */
+FPA_API size_t fpa_decode_workspace_bytes(const FpaCache* cache, int B, int n, int prefix_len);
 
 #ifdef __cplusplus
 }
