@@ -6,15 +6,18 @@
 // sum, and each score is one subtraction and one division, rounded once each: the token does not depend on how the
 // vocabulary is cut up.
 //
-// Bound by the bytes of three rows of V per sequence. A cluster of CTAs shares a sequence; every CTA finds `a` itself
-// (a few gathers), takes a part of the vocabulary and leaves its best (score, index) in shared memory, which the first
-// CTA compares through distributed shared memory.
+// Bound by the bytes of three rows of V per sequence, and by latency when sequences are few: a cluster of CTAs shares a
+// sequence, every CTA finds `a` itself (a few gathers), takes a part of the vocabulary with eight entries' loads in
+// flight per thread, and leaves its best (score, index) in shared memory, which all compare through distributed shared
+// memory. A thread divides only where w > 0.999 best e, without which w / e cannot reach its best so far. The target's
+// own scores are looked at in a second pass, in the rare case that the first finds nothing.
 #include "fpa_serve.h"
 
 namespace fpa {
 namespace {
 
 constexpr int kThreads = 512;
+constexpr int kAhead = 8;  // entries whose loads a thread has in flight
 
 struct VerifyParams {
   const void* p;
@@ -32,14 +35,45 @@ struct VerifyParams {
   int n, V;
 };
 
-// Scores are >= 0, so their bits order as they do; the complement of the index lets the lowest index win a tie.
-__device__ __forceinline__ unsigned long long key_of(float w, float e, int v) {
-  const float score = __fdiv_rn(w, e);
-  if (!(w > 0.f) || !(score >= 0.f)) return 0ull;
-  return (static_cast<unsigned long long>(__float_as_uint(score) + 1u) << 32) | (0xffffffffu - unsigned(v));
+// Best score of the thread's entries v = first, first + step, ... of the row w = pr - qr (qr null: pr) over e, as a key:
+// scores are >= 0, so their bits order as they do; the complement of the index lets the lowest index win a tie.
+template <typename T>
+__device__ __forceinline__ unsigned long long scan_row(const T* pr, const T* qr, const float* e, int V, int first, int step) {
+  float best = 0.f;
+  unsigned long long key = 0;
+  for (int v0 = first; v0 < V; v0 += kAhead * step) {
+    float w[kAhead], n[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int v = v0 + i * step;
+      w[i] = n[i] = 0.f;
+      if (v < V) {
+        w[i] = to_f32(pr[v]);
+        n[i] = e[v];
+      }
+    }
+    if (qr) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int v = v0 + i * step;
+        if (v < V) w[i] = __fsub_rn(w[i], to_f32(qr[v]));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (w[i] > 0.f && !(w[i] < best * n[i] * 0.999f)) {
+        const float score = __fdiv_rn(w[i], n[i]);
+        if (score > best || (key == 0 && score >= 0.f)) {  // a later index never wins a tie
+          best = score;
+          key = (static_cast<unsigned long long>(__float_as_uint(score) + 1u) << 32) | (0xffffffffu - unsigned(v0 + i * step));
+        }
+      }
+    }
+  }
+  return key;
 }
 
-// Best key of the block (in every thread of warp 0); `red` holds one key per warp.
+// Best key of the block, in every thread; `red` holds one key per warp.
 __device__ __forceinline__ unsigned long long block_best(unsigned long long k, unsigned long long* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
@@ -57,7 +91,7 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ VerifyParams a) {
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ VerifyParams a) {
   __shared__ unsigned long long red[kThreads / 32], best[2];
   __shared__ int first;
   pdl_wait();
@@ -85,40 +119,31 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
   __syncthreads();
   const int acc = first;
   const T* pr = P + acc * a.pt;
-  const T* qr = acc < n ? Q + acc * a.qt : nullptr;
+  const T* qr = acc < n ? Q + acc * a.qt : nullptr;  // all accepted: the target's own probabilities
   const float* e = a.noise + b * a.nb;
-  // The residual's best and, for a residual of nothing, the target's own best.
-  unsigned long long kr = 0, kp = 0;
-  for (int v = rank * kThreads + int(threadIdx.x); v < a.V; v += S * kThreads) {
-    const float pv = to_f32(pr[v]), ev = e[v];
-    if (qr) {
-      kr = max(kr, key_of(__fsub_rn(pv, to_f32(qr[v])), ev, v));
+  // The best of the residual; where it is nowhere positive, of the target's probabilities.
+  unsigned long long k = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1) {
+      if (k || !qr) break;  // the same in every thread of the cluster
+      qr = nullptr;
     }
-    kp = max(kp, key_of(pv, ev, v));
-  }
-  kr = block_best(kr, red);
-  kp = block_best(kp, red);
-  if (threadIdx.x == 0) {
-    best[0] = kr;
-    best[1] = kp;
-  }
-  if (S > 1) {
-    cluster_sync();
-    if (rank == 0 && threadIdx.x == 0) {
-      for (int c = 1; c < S; ++c) {
+    k = block_best(scan_row(pr, qr, e, a.V, rank * kThreads + int(threadIdx.x), S * kThreads), red);
+    if (S > 1) {
+      if (threadIdx.x == 0) best[pass] = k;
+      cluster_sync();
+      k = 0;
+      for (int c = 0; c < S; ++c) {
         uint32_t at;
-        unsigned long long x, y;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(best))), "r"(c));
+        unsigned long long x;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(best + pass))), "r"(c));
         asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(at) : "memory");
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(y) : "r"(at + 8) : "memory");
-        kr = max(kr, x);
-        kp = max(kp, y);
+        k = max(k, x);
       }
+      cluster_sync();
     }
-    cluster_sync();
   }
   if (rank == 0 && threadIdx.x < 32) {
-    const unsigned long long k = __shfl_sync(0xffffffffu, kr ? kr : kp, 0);
     // Nothing positive anywhere (all zeros or NaN): the lowest index.
     const int64_t next = k ? int64_t(0xffffffffu - unsigned(k)) : 0;
     for (int i = threadIdx.x; i <= a.n; i += 32)
@@ -150,9 +175,10 @@ extern "C" FPA_API int fpa_verify(const FpaVerifyArgs* a, void* stream) {
   VerifyParams p{a->p, a->q, a->p_stride[0], a->p_stride[1], a->q_stride[0], a->q_stride[1], a->draft, a->draft_stride[0],
                  a->draft_stride[1], a->u, a->u_stride[0], a->u_stride[1], a->noise, a->noise_stride, a->draft_lens,
                  a->accepted, a->tokens, a->n, a->V};
-  // Up to 8 CTAs for a sequence, while the grid leaves SMs idle and every thread keeps an entry.
+  // Up to 8 CTAs for a sequence, while all CTAs run at once (two on an SM) and every thread keeps an entry. For 64
+  // sequences of 50304 entries, two waves of CTAs take 36 us.
   int S = 1;
-  while (S < 8 && a->B * S < 2 * sm_count() && S * kThreads < a->V) S *= 2;
+  while (S < 8 && a->B * S <= sm_count() && S * kThreads < a->V) S *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(S, a->B);
   cfg.blockDim = dim3(kThreads);
