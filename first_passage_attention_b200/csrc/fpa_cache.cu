@@ -3,7 +3,10 @@
 // Both are one pass over the data and bound by its bytes. Eight elements of a row belong to one lane (16 bytes of
 // fp16), D / 8 lanes to a row. int8: the row's largest magnitude `top` by shuffles, scale = top / 127, code =
 // rint((127 x) / top): for fp16 inputs 127 x is exact in float32 and the quotient of two 18- and 11-bit integers never
-// comes closer to a half without being one than float32 resolves, so every code is the correctly rounded one.
+// comes closer to a half without being one than float32 resolves, so every code is the correctly rounded one. The
+// quotient is taken as a product with 1 / top, which is off by less than 2^-14 for |quotient| <= 127, and as a division
+// only where the product lies that close to a half. Stored is code + 128. Each thread has the loads of several rows in
+// flight before it works on the first.
 // A block of the append owns one page of one (sequence, head): it alone writes the page's minimum of phi.
 #include "fpa_serve.h"
 
@@ -11,6 +14,7 @@ namespace fpa {
 namespace {
 
 constexpr int kThreads = 128;
+constexpr int kAhead = 4;  // rows whose loads a thread has in flight
 
 // Eight consecutive elements of a row in float32.
 template <typename T>
@@ -99,40 +103,55 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   const int sub = threadIdx.x / lanes, e0 = (threadIdx.x - sub * lanes) * 8;
   const int tokens = i1 - i0;
   // Rows 0 .. tokens - 1 are K's, the rest V's. Whole warps stay in the loop for the shuffles.
-  for (int r0 = 0; r0 < 2 * tokens; r0 += rows) {
-    const int r = r0 + sub;
-    const bool ok = r < 2 * tokens;
-    const int which = ok && r >= tokens ? 1 : 0, i = ok ? r - which * tokens : 0;
-    float x[8];
+  for (int r0 = 0; r0 < 2 * tokens; r0 += kAhead * rows) {
+    float x[kAhead][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (ok) {
-      const Str4& st = p.st[which];
-      load8(static_cast<const T*>(p.src[which]) + b * st.b + h * st.h + (i0 + i) * st.t + e0 * st.d, st.d,
-            p.vec[which] != 0, x);
+    for (int a = 0; a < kAhead; ++a) {
+      const int r = r0 + a * rows + sub;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[a][j] = 0.f;
+      if (r < 2 * tokens) {
+        const int which = r >= tokens ? 1 : 0;
+        const Str4& st = p.st[which];
+        load8(static_cast<const T*>(p.src[which]) + b * st.b + h * st.h + (i0 + r - which * tokens) * st.t + e0 * st.d,
+              st.d, p.vec[which] != 0, x[a]);
+      }
     }
-    const int64_t at = base + slot0 + i;
-    if constexpr (kInt8) {
-      float top = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
-      for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // Scales stay at or above 2^-90, so that their inverses sum up in float32 (see fpa_decode_mma.cu); a row of
-      // zeros takes that smallest scale, so that it does not outweigh small rows there.
-      top = fmaxf(top, 127.f * 0x1p-90f);
-      uint32_t w[2] = {0, 0};
+    for (int a = 0; a < kAhead; ++a) {
+      if (r0 + a * rows >= 2 * tokens) break;
+      const int r = r0 + a * rows + sub;
+      const bool ok = r < 2 * tokens;
+      const int which = ok && r >= tokens ? 1 : 0;
+      const int64_t at = base + slot0 + r - which * tokens;
+      if constexpr (kInt8) {
+        float top = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int code = min(max(__float2int_rn(__fdiv_rn(__fmul_rn(x[j], 127.f), top)), -127), 127);
-        w[j >> 2] |= uint32_t(code & 0xff) << (8 * (j & 3));
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[a][j]));
+        for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // Scales stay at or above 2^-90, so that their inverses sum up in float32 (see fpa_decode_mma.cu); a row of
+        // zeros takes that smallest scale, so that it does not outweigh small rows there.
+        top = fmaxf(top, 127.f * 0x1p-90f);
+        const float inv = __frcp_rn(top);
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float y = __fmul_rn(x[a][j], 127.f);
+          float c_ = __fmul_rn(y, inv);
+          int code = __float2int_rn(c_);
+          // Near a half, or with a reciprocal or product out of float32's normal range: the division itself.
+          if (!(fabsf(fabsf(c_ - float(code)) - 0.5f) > 0x1p-13f) || !(top < 0x1p100f))
+            code = min(max(__float2int_rn(__fdiv_rn(y, top)), -127), 127);
+          w[j >> 2] |= uint32_t(code + 128) << (8 * (j & 3));
+        }
+        if (ok) {
+          char* dst = const_cast<char*>(static_cast<const char*>(which ? c.v : c.k)) + at * c.D + e0;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+          if (e0 == 0) const_cast<float*>(which ? c.vs : c.ks)[at] = __fdiv_rn(top, 127.f);
+        }
+      } else if (ok) {
+        store8(const_cast<T*>(static_cast<const T*>(which ? c.v : c.k)) + at * c.D + e0, x[a]);
       }
-      if (ok) {
-        char* dst = const_cast<char*>(static_cast<const char*>(which ? c.v : c.k)) + at * c.D + e0;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-        if (e0 == 0) const_cast<float*>(which ? c.vs : c.ks)[at] = __fdiv_rn(top, 127.f);
-      }
-    } else if (ok) {
-      store8(const_cast<T*>(static_cast<const T*>(which ? c.v : c.k)) + at * c.D + e0, x);
     }
   }
   // The field, and the page's minimum over the slots up to the last one written.
@@ -203,26 +222,46 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
   };
   const int lanes = c.D >> 3, rows = kThreads / lanes;
   const int sub = threadIdx.x / lanes, e0 = (threadIdx.x - sub * lanes) * 8;
-  for (int i = i0 + sub; i < i1; i += rows) {
-    const int64_t at = slot(i);
+  for (int first = i0 + sub; first < i1; first += kAhead * rows) {
+    int64_t at[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) at[a] = first + a * rows < i1 ? slot(first + a * rows) : -1;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      float x[8];
+      const void* src = which ? c.v : c.k;
+      T* dst = static_cast<T*>(which ? p.v : p.k) + (out0 + first) * c.D + e0;
+      if constexpr (kInt8) {
+        uint2 w[kAhead];
+        float scale[kAhead];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.f;
-      if (at >= 0) {
-        const void* src = which ? c.v : c.k;
-        if constexpr (kInt8) {
-          const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const char*>(src) + at * c.D + e0);
-          const float scale = (which ? c.vs : c.ks)[at];
+        for (int a = 0; a < kAhead; ++a) {
+          w[a] = make_uint2(0, 0);
+          scale[a] = 0.f;
+          if (at[a] >= 0) {
+            w[a] = __ldcs(reinterpret_cast<const uint2*>(static_cast<const char*>(src) + at[a] * c.D + e0));
+            scale[a] = (which ? c.vs : c.ks)[at[a]];
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          float x[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            x[j] = float(static_cast<signed char>((j < 4 ? w.x : w.y) >> (8 * (j & 3)))) * scale;
-        } else {
-          load8(static_cast<const T*>(src) + at * c.D + e0, 1, true, x);
+            x[j] = at[a] >= 0 ? float(int(((j < 4 ? w[a].x : w[a].y) >> (8 * (j & 3))) & 0xff) - 128) * scale[a] : 0.f;
+          if (first + a * rows < i1) store8(dst + int64_t(a) * rows * c.D, x);
         }
+      } else {
+        float x[kAhead][8];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[a][j] = 0.f;
+          if (at[a] >= 0) load8(static_cast<const T*>(src) + at[a] * c.D + e0, 1, true, x[a]);
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+          if (first + a * rows < i1) store8(dst + int64_t(a) * rows * c.D, x[a]);
       }
-      store8(static_cast<T*>(which ? p.v : p.k) + (out0 + i) * c.D + e0, x);
     }
   }
   for (int i = i0 + threadIdx.x; i < i1; i += kThreads) {

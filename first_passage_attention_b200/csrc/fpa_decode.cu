@@ -12,14 +12,6 @@ int invalid(const char* msg) {
   return FPA_ERR_INVALID_ARGUMENT;
 }
 
-// CTAs that share the history of one (sequence, head): the cluster size, a power of two up to 8 (the portable limit).
-// Doubled until the grid has about four CTAs for every SM, as long as every warp keeps at least two 32-key tiles.
-int own_splits(int64_t units, int64_t max_len) {
-  int s = 1;
-  while (s < 8 && units * s < 4 * sm_count() && max_len >= int64_t(s) * 2 * 4 * 64) s *= 2;
-  return s;
-}
-
 // Parts of the prefix: enough CTAs for four per SM, at least two 32-key tiles for each of their four warps.
 int prefix_parts(int64_t units, int prefix_len) {
   const int64_t most = (int64_t(prefix_len) + 255) / 256;
@@ -105,7 +97,7 @@ extern "C" FPA_API int fpa_decode(FpaDecodeArgs* a, void* stream) {
     e = launch_row_min(p, s);
     if (e == cudaSuccess) {
       prof_mark(s, "decode_prefix");
-      e = run(p, i8, true, p.chunks, s);
+      e = run(p, i8, true, s);
     }
     if (e != cudaSuccess) {
       set_last_error(std::string("fpa_decode, prefix: ") + cudaGetErrorString(e));
@@ -113,9 +105,8 @@ extern "C" FPA_API int fpa_decode(FpaDecodeArgs* a, void* stream) {
     }
     a->kernels_launched = 2;
   }
-  const int64_t max_len = int64_t(p.max_pages) * c.page_size;
   prof_mark(s, "decode");
-  e = run(p, i8, false, own_splits(int64_t(p.B) * c.H, max_len), s);
+  e = run(p, i8, false, s);
   prof_mark(s, nullptr);
   if (e != cudaSuccess) {
     set_last_error(std::string("fpa_decode: ") + cudaGetErrorString(e));

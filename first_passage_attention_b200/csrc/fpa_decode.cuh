@@ -7,8 +7,9 @@
 // the pairs among the n newest tokens get their minimum one by one. A prefix shared by the batch is the same thing once
 // more: its keys' SUF ends at the prefix's end and M_r is the minimum over the row's own tokens.
 //
-// What bounds it: the bytes of the cache. A CTA of four warps takes a (sequence, head, row group) or, as one of up to
-// 8 CTAs of a cluster, a part of its history; every warp walks its own consecutive run of 32-key tiles from the latest
+// What bounds it: the bytes of the cache, and for short histories a chain of look-ups (length, table, values) of about
+// 2 us. A CTA of up to four warps takes a (sequence, head, row group) or, as one of up to 8 CTAs of a cluster, a part
+// of its history; every warp walks its own consecutive run of 16- or 32-key blocks from the latest
 // to the earliest, so that SUF is a running minimum that the warp carries in a register, and no warp waits for
 // another until the end. What lies after a warp's run enters through the page minima (phi_min), four bytes a page and
 // head. The softmax states (m, l, O) of the warps join in shared memory, those of the cluster's CTAs through
@@ -19,46 +20,69 @@
 
 namespace fpa {
 
-// The warp's minimum of phi over the positions [from, to) of a sequence: whole pages through phi_min, the rest from
-// phi itself.
-__device__ __forceinline__ float later_min(const CacheView& c, const int32_t* table, int h, int from, int to) {
-  const int lane = threadIdx.x & 31, page = 1 << c.page_shift;
-  float x = kInf;
-  const int e1 = min(to, (from + page - 1) & -page);
-  const int p1 = to >> c.page_shift;
-  const int e2 = max(e1, p1 << c.page_shift);
-  if (from < e1) {
-    const int pid = table[from >> c.page_shift];
-    if (unsigned(pid) < unsigned(c.n_pages)) {
-      const float* f = c.phi + ((int64_t(pid) * c.H + h) << c.page_shift);
-      for (int s = from + lane; s < e1; s += 32) x = fminf(x, f[s & (page - 1)]);
-    }
-  }
-  for (int pg = (e1 >> c.page_shift) + lane; pg < p1; pg += 32) {
-    const int pid = table[pg];
-    if (unsigned(pid) < unsigned(c.n_pages)) x = fminf(x, c.pmin[int64_t(pid) * c.H + h]);
-  }
-  if (e2 < to) {
-    const int pid = table[e2 >> c.page_shift];
-    if (unsigned(pid) < unsigned(c.n_pages)) {
-      const float* f = c.phi + ((int64_t(pid) * c.H + h) << c.page_shift);
-      for (int s = e2 + lane; s < to; s += 32) x = fminf(x, f[s & (page - 1)]);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x = fminf(x, __shfl_xor_sync(0xffffffffu, x, o));
-  return x;
-}
+constexpr int kMaxWarps = 4;  // of a CTA
 
-// Index of slot `pos` of head h in the pool's [n_pages, H, page_size] arrays, or -1 where the table's entry lies
-// outside the pool (recorded in the status word).
-__device__ __forceinline__ int64_t slot_of(const CacheView& c, const int32_t* table, int h, int pos) {
-  const int pid = table[pos >> c.page_shift];
+// Index of slot `pos` of head h in the pool's [n_pages, H, page_size] arrays, given its page's id, or -1 where the id
+// lies outside the pool (recorded in the status word).
+__device__ __forceinline__ int64_t slot_in(const CacheView& c, int pid, int h, int pos) {
   if (unsigned(pid) >= unsigned(c.n_pages)) {
     report_bad_page(c.status, kSiteDecode);
     return -1;
   }
   return ((int64_t(pid) * c.H + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+}
+__device__ __forceinline__ int64_t slot_of(const CacheView& c, const int32_t* table, int h, int pos) {
+  return slot_in(c, table[pos >> c.page_shift], h, pos);
+}
+
+// The warp's minimum of phi over the positions [from, to) of a sequence: whole pages through phi_min, the rest from
+// phi itself. In three steps, so that the table's entries, and then the values, of this and of the caller's other
+// look-ups travel together.
+struct LaterMin {
+  int from, to, e1, e2, p0, p1;  // [from, e1) of a first page, pages p0 .. p1 - 1, [e2, to) of a last page
+  int pid_a, pid_p, pid_z;
+  float x;
+
+  __device__ __forceinline__ void ids(const CacheView& c, const int32_t* table, int from_, int to_) {
+    const int lane = threadIdx.x & 31, page = 1 << c.page_shift;
+    from = from_;
+    to = max(from_, to_);
+    e1 = min(to, (from + page - 1) & -page);
+    p0 = e1 >> c.page_shift;
+    p1 = max(p0, to >> c.page_shift);
+    e2 = max(e1, p1 << c.page_shift);
+    pid_a = from < e1 ? table[from >> c.page_shift] : -1;
+    pid_p = p0 + lane < p1 ? table[p0 + lane] : -1;
+    pid_z = e2 < to ? table[e2 >> c.page_shift] : -1;
+  }
+  __device__ __forceinline__ static float part(const CacheView& c, int pid, int h, int s0, int s1) {
+    float x = kInf;
+    if (unsigned(pid) < unsigned(c.n_pages)) {
+      const float* f = c.phi + ((int64_t(pid) * c.H + h) << c.page_shift);
+      for (int s = s0 + (threadIdx.x & 31); s < s1; s += 32) x = fminf(x, f[s & ((1 << c.page_shift) - 1)]);
+    }
+    return x;
+  }
+  __device__ __forceinline__ void values(const CacheView& c, int h) {
+    x = unsigned(pid_p) < unsigned(c.n_pages) ? c.pmin[int64_t(pid_p) * c.H + h] : kInf;
+    x = fminf(x, fminf(part(c, pid_a, h, from, e1), part(c, pid_z, h, e2, to)));
+  }
+  __device__ __forceinline__ float finish(const CacheView& c, const int32_t* table, int h) {
+#pragma unroll 4
+    for (int pg = p0 + 32 + (threadIdx.x & 31); pg < p1; pg += 32) {
+      const int pid = table[pg];
+      if (unsigned(pid) < unsigned(c.n_pages)) x = fminf(x, c.pmin[int64_t(pid) * c.H + h]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = fminf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+  }
+};
+__device__ __forceinline__ float later_min(const CacheView& c, const int32_t* table, int h, int from, int to) {
+  LaterMin m;
+  m.ids(c, table, from, to);
+  m.values(c, h);
+  return m.finish(c, table, h);
 }
 
 // Minimum over the lanes' x of the lanes strictly after this one (+inf for lane 31); `all` gets the warp's minimum.
@@ -88,20 +112,19 @@ __device__ __forceinline__ float prefix_min(float x) {
 // The newest tokens of a sequence, one per lane (lanes >= nn hold nothing).
 struct NewTokens {
   float phi, psi;  // +inf, 0 on the empty lanes
-  float low;       // min of phi over the new tokens up to this lane's
+  float low;       // min of phi over the new tokens up to this lane's (filled by the caller: prefix_min(phi))
   int64_t slot;    // pool index, or -1
   int nn;
 };
 
-__device__ __forceinline__ NewTokens load_new(const CacheView& c, const int32_t* table, int h, int Lb, int nn) {
+__device__ __forceinline__ NewTokens load_new(const CacheView& c, int pid, int h, int Lb, int nn) {
   const int lane = threadIdx.x & 31;
   NewTokens t{kInf, 0.f, kInf, -1, nn};
-  if (lane < nn) t.slot = slot_of(c, table, h, Lb + lane);
+  if (lane < nn) t.slot = slot_in(c, pid, h, Lb + lane);
   if (t.slot >= 0) {
     t.phi = c.phi[t.slot];
     t.psi = c.psi[t.slot];
   }
-  t.low = prefix_min(t.phi);
   return t;
 }
 
@@ -124,7 +147,7 @@ struct Job {
   int rows;           // rows of this group
   int r0;             // first row: of the sequence's n (decode) or of the head's R (prefix)
   int end;            // history keys [0, end)
-  int t0, t1;         // this warp's tiles of 32 keys
+  int t0, t1;         // this warp's blocks of Core::kKeys keys
   int n_new;          // new tokens in the cache (decode)
   int lead;           // rows of the sequence that stand before its first token
   bool last;          // this warp also takes the tile of the new tokens
@@ -148,23 +171,31 @@ __device__ __forceinline__ void cluster_barrier() {
 // Weight of a softmax state with maximum m in a joint one with maximum M (0 for an empty state).
 __device__ __forceinline__ float state_weight(float m, float M) { return m == -kInf ? 0.f : ex2(m - M); }
 
+// Dynamic shared memory of a CTA: the warps' rings, whose place the joining of their states takes over at the end;
+// the cores' scratch, of the CTA and of each warp; the states' maxima and sums.
 template <class Core>
-constexpr int decode_smem_floats() {
-  return ((Core::W * Core::NQ * (2 + Core::D) + 2 * Core::NQ + 3) & -4) + Core::kScratchFloats;
+__host__ __device__ constexpr int decode_warp_bytes() {
+  return Core::kRingBytes > Core::NQ * Core::D * 4 ? Core::kRingBytes : Core::NQ * Core::D * 4;
+}
+template <class Core>
+__host__ __device__ constexpr int decode_smem_bytes(int warps) {
+  return warps * decode_warp_bytes<Core>() +
+         (Core::kCtaFloats + warps * (Core::kWarpFloats + 2 * Core::NQ) + 2 * Core::NQ) * 4;
 }
 
 // Core: the arithmetic of one warp over a run of keys (see fpa_decode_mma.cu, fpa_decode_ffma.cu).
 // kPrefix: the rows (b, i) of the whole batch against the prefix, partial results to the workspace.
 template <class Core, bool kPrefix>
-__global__ void __launch_bounds__(Core::W * 32, Core::kMinBlocks) decode_kernel(const __grid_constant__ DecodeParams p) {
-  extern __shared__ __align__(16) float smem[];
-  constexpr int W = Core::W, NQ = Core::NQ, D = Core::D;
+__global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kernel(const __grid_constant__ DecodeParams p) {
+  extern __shared__ __align__(128) float smem[];
+  constexpr int NQ = Core::NQ, D = Core::D;
+  const int W = blockDim.x >> 5;
   float* sO = smem;                 // [W][NQ][D]
-  float* sm = sO + W * NQ * D;      // [W][NQ]
+  float* scratch = smem + W * (decode_warp_bytes<Core>() / 4);
+  float* sm = scratch + Core::kCtaFloats + W * Core::kWarpFloats;  // [W][NQ]
   float* sl = sm + W * NQ;          // [W][NQ]
   float* cm = sl + W * NQ;          // [NQ]
   float* cl = cm + NQ;              // [NQ]
-  float* scratch = smem + ((W * NQ * (2 + D) + 2 * NQ + 3) & -4);
   const int warp = threadIdx.x >> 5;
   const int S = gridDim.x, rank = blockIdx.x;
   // A prefix pass before this kernel has waited for everything before it, so only its own results are still open:
@@ -203,14 +234,15 @@ __global__ void __launch_bounds__(Core::W * 32, Core::kMinBlocks) decode_kernel(
   job.rows = min(NQ, R - job.r0);
   job.bias = p.beta[job.h] * kLog2e;
   {
-    const int tiles = (job.end + 31) >> 5, units = S * W, u = rank * W + warp;
+    const int tiles = (job.end + Core::kKeys - 1) / Core::kKeys, units = S * W, u = rank * W + warp;
     const int each = tiles / units, more = tiles - each * units;
     job.t0 = u * each + min(u, more);
     job.t1 = job.t0 + each + (u < more ? 1 : 0);
     job.last = !kPrefix && u == units - 1;
   }
-  Core core(p, job, scratch);
+  Core core(p, job, scratch, reinterpret_cast<char*>(smem));
   core.template run<kPrefix>(p, job);
+  if (Core::kRingBytes > 0) __syncthreads();  // every warp is done with its ring
   core.store(sm + warp * NQ, sl + warp * NQ, sO + warp * NQ * D, job.rows);
   __syncthreads();
   // The CTA's state: maxima and sums per row, O in the first warp's place.
@@ -226,7 +258,6 @@ __global__ void __launch_bounds__(Core::W * 32, Core::kMinBlocks) decode_kernel(
     const int r = e / D;
     const float M = cm[r];
     float o = 0.f;
-#pragma unroll
     for (int w = 0; w < W; ++w) o += sO[w * NQ * D + e] * state_weight(sm[w * NQ + r], M);
     if constexpr (kPrefix) {
       const int64_t at = (int64_t(job.h) * R + job.r0 + r) * p.chunks + rank;
@@ -273,15 +304,31 @@ __global__ void __launch_bounds__(Core::W * 32, Core::kMinBlocks) decode_kernel(
   }
 }
 
-// Grid and launch of one pass. splits: CTAs of a cluster (own tokens) or parts of the prefix.
+// Grid and launch of one pass. chunks (prefix): CTAs that share the prefix.
+//
+// CTAs of four warps for each (sequence, head, row group): as many as make two rounds of CTAs on the GPU, up to the 8 of
+// a cluster, and at least a block for each warp. Fewer leave SMs unevenly loaded at the end, more pay the start-up
+// chain too often (64 units of 16383 tokens, fp16 D = 128: 3 CTAs each 82 us, 4 to 6 70-71, 8, which is two rounds, 68;
+// 768 units of up to 2048, int8 D = 64: 34.3 us with one, 38.7 with two).
 template <class Core>
-cudaError_t launch_decode_core(DecodeParams p, bool prefix, int splits, cudaStream_t s) {
-  constexpr int smem = decode_smem_floats<Core>() * 4;
+cudaError_t launch_decode_core(DecodeParams p, bool prefix, cudaStream_t s) {
   const int rows = prefix ? p.B * p.n : p.n;
   p.groups = (rows + Core::NQ - 1) / Core::NQ;
+  const int by_regs = Core::kMinBlocks * kMaxWarps, by_smem = (227 * 1024) / decode_smem_bytes<Core>(1);
+  const int64_t slots = int64_t(sm_count()) * (by_regs < by_smem ? by_regs : by_smem);
+  const int64_t units = int64_t(p.c.H) * p.groups * (prefix ? 1 : p.B);
+  const int64_t len = prefix ? p.prefix_len : int64_t(p.max_pages) << p.c.page_shift;
+  const int64_t blocks = (len + Core::kKeys - 1) / Core::kKeys;
+  int W = int(blocks < kMaxWarps ? blocks : kMaxWarps), splits = p.chunks;
+  if (!prefix) {
+    int64_t most = 2 * slots / (units * W);
+    if (most > blocks / W) most = blocks / W;
+    splits = int(most < 1 ? 1 : most > 8 ? 8 : most);
+  }
+  const int smem = decode_smem_bytes<Core>(W);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = prefix ? dim3(splits, p.groups, p.c.H) : dim3(splits, p.c.H * p.groups, p.B);
-  cfg.blockDim = dim3(Core::W * 32);
+  cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];

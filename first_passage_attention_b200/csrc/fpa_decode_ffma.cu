@@ -11,12 +11,13 @@ namespace {
 
 template <int D_, bool kInt8, int NR>
 struct FfmaCore {
-  static constexpr int D = D_, W = 4, NQ = NR;
+  static constexpr int D = D_, NQ = NR;
   static constexpr int CPL = D < 32 ? 1 : D / 32;   // columns of V for a lane
   static constexpr int CV = CPL < 4 ? CPL : 4;      // ... of one load
   static constexpr int KG = D < 32 ? 32 / D : 1;    // lanes that share a column take every KG-th key
   static constexpr int kMinBlocks = NR * CPL + D / 4 <= 64 ? 4 : 2;
-  static constexpr int kScratchFloats = NR * D + W * NR * 32;
+  static constexpr int kKeys = 32, kRingBytes = 0;
+  static constexpr int kCtaFloats = NR * D, kWarpFloats = NR * 32;
   using Out = float;
 
   float o[NR][CPL], m[NR], l[NR];
@@ -24,7 +25,7 @@ struct FfmaCore {
   float* ss;  // [NR][32], this warp's scores and probabilities
   int lane, g, t;
 
-  __device__ __forceinline__ FfmaCore(const DecodeParams&, const Job&, float* scratch) {
+  __device__ __forceinline__ FfmaCore(const DecodeParams&, const Job&, float* scratch, char*) {
     lane = threadIdx.x & 31;
     g = lane >> 2;
     t = lane & 3;
@@ -37,8 +38,8 @@ struct FfmaCore {
   // Four elements d .. d + 3 of the key at pool index `slot` (codes for int8).
   __device__ __forceinline__ static float4 load4(const void* base, int64_t slot, int d) {
     if constexpr (kInt8) {
-      const char4 x = __ldg(reinterpret_cast<const char4*>(static_cast<const char*>(base) + slot * D + d));
-      return make_float4(x.x, x.y, x.z, x.w);
+      const uchar4 x = __ldg(reinterpret_cast<const uchar4*>(static_cast<const char*>(base) + slot * D + d));
+      return make_float4(x.x - 128, x.y - 128, x.z - 128, x.w - 128);
     } else {
       return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + slot * D + d));
     }
@@ -56,7 +57,7 @@ struct FfmaCore {
 #pragma unroll
       for (int j = 0; j < CPL; ++j) {
         const int64_t at = slot * D + (D < 32 ? (threadIdx.x & (D - 1)) : column(j));
-        v[j] = kInt8 ? float(__ldg(static_cast<const signed char*>(base) + at)) : __ldg(static_cast<const float*>(base) + at);
+        v[j] = kInt8 ? float(__ldg(static_cast<const unsigned char*>(base) + at) - 128) : __ldg(static_cast<const float*>(base) + at);
       }
     }
   }
@@ -146,7 +147,7 @@ struct FfmaCore {
   template <bool kPrefix>
   __device__ __forceinline__ void run(const DecodeParams& p, const Job& job) {
     const CacheView& c = p.c;
-    for (int e = threadIdx.x; e < NR * D; e += W * 32) {
+    for (int e = threadIdx.x; e < NR * D; e += blockDim.x) {
       const int r = e / D, d = e - r * D;
       float x = 0.f;
       if (r < job.rows) {
@@ -161,7 +162,10 @@ struct FfmaCore {
     }
     __syncthreads();
     NewTokens nw{kInf, 0.f, kInf, -1, 0};
-    if constexpr (!kPrefix) nw = load_new(c, job.table, job.h, job.end, job.n_new);
+    if constexpr (!kPrefix) {
+      nw = load_new(c, lane < job.n_new ? job.table[(job.end + lane) >> c.page_shift] : -1, job.h, job.end, job.n_new);
+      nw.low = prefix_min(nw.phi);
+    }
     float low[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
@@ -253,14 +257,14 @@ struct FfmaCore {
 };
 
 template <bool kInt8>
-cudaError_t launch_for(const DecodeParams& p, bool prefix, int splits, cudaStream_t s) {
+cudaError_t launch_for(const DecodeParams& p, bool prefix, cudaStream_t s) {
   const int rows = prefix ? p.B * p.n : p.n;
   switch (p.c.D) {
 #define FPA_CASE(D)                                                                                  \
   case D:                                                                                            \
-    return rows == 1  ? launch_decode_core<FfmaCore<D, kInt8, 1>>(p, prefix, splits, s)              \
-           : rows < 5 ? launch_decode_core<FfmaCore<D, kInt8, 4>>(p, prefix, splits, s)              \
-                      : launch_decode_core<FfmaCore<D, kInt8, 8>>(p, prefix, splits, s);
+    return rows == 1  ? launch_decode_core<FfmaCore<D, kInt8, 1>>(p, prefix, s)              \
+           : rows < 5 ? launch_decode_core<FfmaCore<D, kInt8, 4>>(p, prefix, s)              \
+                      : launch_decode_core<FfmaCore<D, kInt8, 8>>(p, prefix, s);
     FPA_CASE(16)
     FPA_CASE(32)
     FPA_CASE(64)
@@ -282,8 +286,13 @@ __global__ void __launch_bounds__(128) row_min_kernel(const __grid_constant__ De
   const int32_t* table = p.table + b * p.table_stride;
   const int cap = int(min(int64_t(p.max_pages) << p.c.page_shift, int64_t(INT32_MAX)));
   const int L = min(max(p.lengths[b], 0), cap), Lb = max(L - p.n, 0), nn = L - Lb, lead = p.n - nn;
-  const NewTokens nw = load_new(p.c, table, h, Lb, nn);
-  const float before = Lb > 0 ? later_min(p.c, table, h, 0, Lb) : kInf;
+  const int pid = lane < nn ? table[(Lb + lane) >> p.c.page_shift] : -1;
+  LaterMin own;
+  own.ids(p.c, table, 0, Lb);
+  NewTokens nw = load_new(p.c, pid, h, Lb, nn);
+  own.values(p.c, h);
+  nw.low = prefix_min(nw.phi);
+  const float before = own.finish(p.c, table, h);
   if (lane < p.n) {
     float* out = p.row_min + int64_t(h) * (p.B * p.n) + b * p.n;
     if (lane < lead) out[lane] = kInf;
@@ -293,8 +302,8 @@ __global__ void __launch_bounds__(128) row_min_kernel(const __grid_constant__ De
 
 }  // namespace
 
-cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, int splits, cudaStream_t s) {
-  return int8 ? launch_for<true>(p, prefix, splits, s) : launch_for<false>(p, prefix, splits, s);
+cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s) {
+  return int8 ? launch_for<true>(p, prefix, s) : launch_for<false>(p, prefix, s);
 }
 
 cudaError_t launch_row_min(const DecodeParams& p, cudaStream_t s) {

@@ -2,19 +2,23 @@
 //
 // The products are S^T = K Q^T (16 keys x 16 d times 16 d x 8 rows) and O^T = V^T P^T (16 d x 16 keys times 16 keys x 8
 // rows): the keys, which are many, fill the instruction's 16 rows, and the query rows, which are few, its 8 columns.
-// With at most 16 rows there are at most 32 flops a byte, a tenth of what would make the tensor cores' rate matter,
-// so the loads decide: the fragments come straight from global memory into registers. Lane (g, t) = (lane / 4, lane
-// % 4) needs, of K, some four elements of key g for each 16-d step: which ones is free as long as Q agrees, so it
-// takes consecutive ones (16 bytes at a time, a full 64-byte run per key and four lanes). Of V it needs, for each 16-d
-// tile, two columns of the keys 2t, 2t + 1, 2t + 8, 2t + 9: it takes D / 8 consecutive columns. P passes from the
-// accumulators' layout to the operand's with movmatrix. No shared memory, no barrier, on the way of K and V.
+// With at most 16 rows there are at most 32 flops a byte, a tenth of what would make the tensor cores' rate matter;
+// the bytes bound it, then the instructions that turn them into fragments. Every warp keeps a ring of its own in
+// shared memory, filled by cp.async kStages - 1 blocks of keys ahead: enough bytes in flight on an SM however few
+// CTAs it holds, no register held by a pending load, and no barrier between warps. Fragments come out with ldmatrix:
+// plain for K; transposed for V, where the transposition of pairs of bytes also brings together the codes of two keys
+// that an int8 fragment needs side by side. The 16-byte chunks of a row are permuted in shared memory so that the
+// eight rows of a matrix lie in different banks. P passes from the accumulators' layout to the operand's with movmatrix.
 //
-// int8: codes become fp16 exactly (0x6400 | (code + 128) is 1152 + code); K's scale multiplies the finished product,
-// and V's goes into the exponent. With lv = log2 vs, P' = 2^(z + lv - m) <= 2^8 for m = max(z + lv) as of its last
-// update, l = sum P' / vs and o = sum P' code / l: the factors fp16 holds are scaled to the largest contribution
-// whatever the scales are, and the cost is that of the plain softmax. P' is rounded to fp16 (2^-11 relative, as the
-// training kernels round P); sums and states stay in fp32. The maximum is updated only when it grows by more than 8
-// (in log2 units), decided by the whole warp.
+// int8: a stored byte is u = code + 128. K's bytes are used as they are: with a zero byte above, u is the fp16
+// subnormal u 2^-24, exactly, and the accumulator starts at -128 2^-24 sum_d q_d, which takes the offset out again;
+// K's scale multiplies the finished product. (The offset's products are of the size of the others: float32 loses
+// nothing that matters.) V's bytes become code exactly (0x6400 | u is 1024 + u), since sums over many keys would
+// cancel; V's scale goes into the exponent. With lv = log2 vs, P' = 2^(z + lv - m) <= 2^8 for m = max(z + lv) as of its
+// last update, l = sum P' / vs and o = sum P' code / l: the factors fp16 holds are scaled to the largest contribution
+// whatever the scales are, at the cost of the plain softmax. P' is rounded to fp16 (2^-11 relative, as the training
+// kernels round P); sums and states stay in fp32. The maximum is updated only when it grows by more than 8 (in log2
+// units), decided by the whole warp.
 #include <cuda_fp16.h>
 
 #include "fpa_decode.cuh"
@@ -34,12 +38,43 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// Four (two) 8 x 8 matrices of 16-bit elements, the rows at the lanes' addresses.
+template <bool kTrans>
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  if constexpr (kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool kTrans>
+__device__ __forceinline__ void ldmatrix2(uint32_t addr, uint32_t (&r)[4]) {
+  if constexpr (kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+}
+
+// 16 (4) bytes to shared memory; zeros without touching the source where `ok` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Two halves from bytes (lo, hi) of codes with 128 added: `sel` picks byte 0 / 1 or 2 / 3 of x.
+// Two codes as halves, from the bytes of x that kSel picks.
 template <uint32_t kSel>
 __device__ __forceinline__ uint32_t codes_to_half2(uint32_t x) {
   const uint32_t y = __byte_perm(x, 0x64646464u, kSel);
@@ -47,87 +82,95 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t x) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// kBytes (2, 4, 8 or a multiple of 16) from global memory that this kernel only reads once.
-template <int kBytes, int kStride>
-__device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
-  if constexpr (kBytes == 2) {
-    unsigned short x;
-    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(x) : "l"(p));
-    w[0] = x;
-  } else if constexpr (kBytes == 4) {
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
-  } else if constexpr (kBytes == 8) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-  } else {
-#pragma unroll
-    for (int j = 0; j < kBytes / 16; ++j)
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(w[4 * j]), "=r"(w[4 * j + 1]), "=r"(w[4 * j + 2]), "=r"(w[4 * j + 3])
-                   : "l"(p + j * kStride));
-  }
-}
-
 template <int D_, bool kInt8, int NT>
 struct MmaCore {
-  static constexpr int D = D_, W = 4, NQ = 8 * NT;
-  static constexpr int ES = kInt8 ? 1 : 2;             // bytes of a stored element
-  static constexpr int KB = D / 4 * ES, KV = KB < 16 ? KB : 16;   // bytes of a key for a lane; of one load
-  static constexpr int VB = D / 8 * ES, VV = VB < 16 ? VB : 16;
-  static constexpr int KW = KB / 4, VW = VB < 4 ? 1 : VB / 4;     // 32-bit words
-  static constexpr int KE = KV / ES, VE = VV / ES;                // elements of one load
+  static constexpr int D = D_, NQ = 8 * NT;
+  static constexpr int ES = kInt8 ? 1 : 2;              // bytes of a stored element
+  static constexpr int RB = D * ES;                     // ... of a row
+  static constexpr int CPR = RB / 16;                   // 16-byte chunks of a row
+  static constexpr int SUB = RB <= 128 ? 2 : 1;         // 16-key blocks handled together
+  static constexpr int kKeys = 16 * SUB;
   static constexpr int KS = D / 16, MT = D / 16;
-  static constexpr int SUB = D * ES <= 128 ? 2 : 1;    // 16-key blocks loaded and worked on at a time
-  static constexpr int STEPS = 2 / SUB;
-  // Registers of the fragments and accumulators decide how many CTAs an SM can hold.
-  static constexpr int kRegs = SUB * (2 * KW + 4 * VW) + NT * (2 * KS + 4 * MT);
-  static constexpr int kMinBlocks = kRegs <= 72 ? 4 : kRegs <= 112 ? 3 : 2;
-  static constexpr int kScratchFloats = W * 32 * 5;
+  static constexpr int kArray = kKeys * RB;             // bytes of K (and of V) in a stage
+  static constexpr int kStage = 2 * kArray + (kInt8 ? 4 : 2) * kKeys * 4;
+  // Two stages leave room for more warps, which gain more than a third stage (fp16 D = 128, 16 heads, 4 x 16383
+  // tokens, 5 rows: 64 us against 69); at D = 256 in fp16 few warps fit either way (48 us with three, 60 with two).
+  static constexpr int kStages = RB < 512 ? 2 : 3;
+  static constexpr int kRingBytes = kStages * kStage;   // of a warp
+  static constexpr int kCtaFloats = 0, kWarpFloats = kKeys * 5;
+  static constexpr int kMinBlocks = D * NT <= 64 ? (RB <= 64 ? 5 : 4) : D * NT <= 128 ? 3 : 2;
   using Out = __half;
 
-  uint32_t kf[SUB][2][KW], vf[SUB][4][VW], qf[NT][KS][2];
-  float o[MT][NT][4], m[NT][2], l[NT][2], low[NT][2];
-  float4* par;  // per key of the tile: a, psi, factor of the product, log2 of V's scale (-inf: no such key)
-  float* rvs;   // 1 / V's scale
-  int g, t;
+  uint32_t qf[NT][KS][2];
+  float o[MT][NT][4], m[NT][2], l[NT][2], low[NT][2], zero[NT][2];
+  float4* par;    // per key of the block: a, psi, factor of the product, log2 of V's scale (-inf: no such key)
+  float* rvs;     // 1 / V's scale
+  uint32_t ring;  // this warp's stages
+  int lane, g, t;
 
-  __device__ __forceinline__ MmaCore(const DecodeParams&, const Job&, float* scratch) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __device__ __forceinline__ MmaCore(const DecodeParams&, const Job&, float* scratch, char* rings) {
+    const int warp = threadIdx.x >> 5;
+    lane = threadIdx.x & 31;
     g = lane >> 2;
     t = lane & 3;
-    par = reinterpret_cast<float4*>(scratch) + warp * 32;
-    rvs = scratch + W * 32 * 4 + warp * 32;
+    par = reinterpret_cast<float4*>(scratch + warp * kWarpFloats);
+    rvs = scratch + warp * kWarpFloats + kKeys * 4;
+    ring = static_cast<uint32_t>(__cvta_generic_to_shared(rings)) + warp * kRingBytes;
   }
 
-  __device__ __forceinline__ void load_k(const CacheView& c, int64_t slot, int sub, int key, int lim) {
-    // Key `key` (of the block's g, g + 8) sits at pool index `slot`; beyond `lim` nothing is touched.
-#pragma unroll
-    for (int i = 0; i < KW; ++i) kf[sub][key][i] = 0;
-    if (key * 8 + g < lim) load_words<KB, 4 * KV>(static_cast<const char*>(c.k) + slot * (D * ES) + t * KV, kf[sub][key]);
+  // Byte offset of 16-byte chunk c of a row: bits of the chunk's number are flipped by the row's place among the eight
+  // rows that a matrix reads at once. Stages start at multiples of 128 bytes and rows are powers of two, so for a
+  // fixed row, chunk c lies at chunk_at(row, c0) ^ 16 (c ^ c0) for any c0 < 8 with c < 8.
+  __device__ __forceinline__ static constexpr int swizzle(int row) {
+    constexpr int kLine = RB < 128 ? 128 / RB : 1, kMask = (CPR < 8 ? CPR : 8) - 1;
+    return (row / kLine) & kMask;
   }
-  __device__ __forceinline__ void load_v(const CacheView& c, int64_t slot, int sub, int i, int lim) {
+  __device__ __forceinline__ static int chunk_at(int row, int c) { return (row * CPR + (c ^ swizzle(row))) * 16; }
+  // Address of chunk (even c) + `odd` of a row whose chunk `odd` is at `at`.
+  __device__ __forceinline__ static uint32_t chunk_from(uint32_t at, int c) { return (at ^ ((c & 7) * 16)) + (c >> 3) * 128; }
+
+  // A block of keys that lie one after the other from pool index `base` on, `lim` of them.
+  __device__ __forceinline__ void fetch(const CacheView& c, uint32_t st, int64_t base, int lim) {
+    const char* k = static_cast<const char*>(c.k) + base * RB + lane * 16;
+    const char* v = static_cast<const char*>(c.v) + base * RB + lane * 16;
+    // The lane's chunk of every 512 bytes: its row moves by whole groups of rows, which flip other bits.
+    const uint32_t at = st + chunk_at(lane / CPR, lane % CPR);
+    if (lim == kKeys) {
 #pragma unroll
-    for (int j = 0; j < VW; ++j) vf[sub][i][j] = 0;
-    if ((i >> 1) * 8 + 2 * t + (i & 1) < lim)
-      load_words<VB, 8 * VV>(static_cast<const char*>(c.v) + slot * (D * ES) + g * VV, vf[sub][i]);
-  }
-  // The blocks of step st of the tile at pool index `base` with `lim` keys.
-  __device__ __forceinline__ void load_k_step(const CacheView& c, int64_t base, int st, int lim) {
-#pragma unroll
-    for (int sub = 0; sub < SUB; ++sub)
-#pragma unroll
-      for (int key = 0; key < 2; ++key) {
-        const int first = (st * SUB + sub) * 16;
-        load_k(c, base + first + key * 8 + g, sub, key, lim - first);
+      for (int i = 0; i < kKeys * CPR; i += 32) {
+        const uint32_t to = (at ^ (swizzle(i / CPR) * 16)) + i * 16;
+        copy16(to, k + i * 16, true);
+        copy16(to + kArray, v + i * 16, true);
       }
-  }
-  __device__ __forceinline__ void load_v_step(const CacheView& c, int64_t base, int st, int lim) {
-#pragma unroll
-    for (int sub = 0; sub < SUB; ++sub)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int first = (st * SUB + sub) * 16;
-        load_v(c, base + first + (i >> 1) * 8 + 2 * t + (i & 1), sub, i, lim - first);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kKeys * CPR; i += 32) {
+        const uint32_t to = (at ^ (swizzle(i / CPR) * 16)) + i * 16;
+        copy16(to, k + i * 16, (i + lane) / CPR < lim);
+        copy16(to + kArray, v + i * 16, (i + lane) / CPR < lim);
       }
+    }
+    if (lane < kKeys) fetch_field(c, st, base + lane, lane < lim);
+  }
+  __device__ __forceinline__ void fetch_field(const CacheView& c, uint32_t st, int64_t slot, bool ok) {
+    const uint32_t at = st + 2 * kArray + lane * 4;
+    copy4(at, c.phi + slot, ok);
+    copy4(at + kKeys * 4, c.psi + slot, ok);
+    if constexpr (kInt8) {
+      copy4(at + 2 * kKeys * 4, c.ks + slot, ok);
+      copy4(at + 3 * kKeys * 4, c.vs + slot, ok);
+    }
+  }
+  // The newest tokens, which may lie in two pages: each key at its own place.
+  __device__ __forceinline__ void fetch_new(const CacheView& c, uint32_t st, const NewTokens& nw) {
+#pragma unroll 1
+    for (int i = 0; i < kKeys * CPR; i += 32) {
+      const int idx = i + lane, row = idx / CPR, ch = idx % CPR, at = chunk_at(row, ch);
+      const int64_t slot = __shfl_sync(0xffffffffu, nw.slot, row & 31);
+      copy16(st + at, static_cast<const char*>(c.k) + (slot < 0 ? 0 : slot) * RB + ch * 16, slot >= 0);
+      copy16(st + kArray + at, static_cast<const char*>(c.v) + (slot < 0 ? 0 : slot) * RB + ch * 16, slot >= 0);
+    }
+    if (lane < kKeys) fetch_field(c, st, nw.slot < 0 ? 0 : nw.slot, nw.slot >= 0);
   }
 
   template <bool kPrefix>
@@ -149,48 +192,112 @@ struct MmaCore {
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const int idx = 4 * s + 2 * w, d = (idx / KE * 4 + t) * KE + idx % KE;
-          uint32_t x;
-          if (p.q_pairs) {
-            x = *reinterpret_cast<const uint32_t*>(row + d);
-          } else {
-            const __half2 h = __halves2half2(row[d * p.sq.d], row[(d + 1) * p.sq.d]);
-            x = *reinterpret_cast<const uint32_t*>(&h);
-          }
-          qf[nt][s][w] = ok ? x : 0u;
+          // fp16: elements 2t, 2t + 1 and 2t + 8, 2t + 9 of the 16; int8: the four that a 32-bit word holds.
+          const int d = s * 16 + (kInt8 ? 4 * t + 2 * w : 2 * t + 8 * w);
+          __half2 x;
+          if (p.q_pairs)
+            x = *reinterpret_cast<const __half2*>(row + d);
+          else
+            x = __halves2half2(row[d * p.sq.d], row[(d + 1) * p.sq.d]);
+          if (!ok) x = __floats2half2_rn(0.f, 0.f);
+          qf[nt][s][w] = *reinterpret_cast<const uint32_t*>(&x);
         }
     }
   }
-
-  // S^T of one 16-key block.
-  __device__ __forceinline__ void scores(int sub, float (&z)[NT][4]) {
+  // What the accumulators of the scores start at, for the rows of this lane's columns.
+  __device__ __forceinline__ void sum_q() {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) z[nt][i] = 0.f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      uint32_t a[4];
+    for (int nt = 0; nt < NT; ++nt) {
       if constexpr (kInt8) {
-        const uint32_t x = kf[sub][0][s] ^ 0x80808080u, y = kf[sub][1][s] ^ 0x80808080u;
-        a[0] = codes_to_half2<0x4140>(x);
-        a[1] = codes_to_half2<0x4140>(y);
-        a[2] = codes_to_half2<0x4342>(x);
-        a[3] = codes_to_half2<0x4342>(y);
-      } else {
-        a[0] = kf[sub][0][2 * s];
-        a[1] = kf[sub][1][2 * s];
-        a[2] = kf[sub][0][2 * s + 1];
-        a[3] = kf[sub][1][2 * s + 1];
-      }
+        float sum = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma16816(z[nt], a, qf[nt][s][0], qf[nt][s][1]);
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const __half2 x = *reinterpret_cast<const __half2*>(&qf[nt][s][w]);
+            sum += __low2float(x) + __high2float(x);
+          }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) zero[nt][c] = -128.f * 0x1p-24f * __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
+      } else {
+        zero[nt][0] = zero[nt][1] = 0.f;
+      }
     }
   }
 
-  // Softmax of N blocks of scores (z + lv in log2 units) and their products with V.
-  template <int N>
-  __device__ __forceinline__ void accumulate(float (&z)[N][NT][4], const float (&rv)[N][2]) {
+  // S^T of one 16-key block (int8: times 2^-24).
+  __device__ __forceinline__ void scores(uint32_t st, int sub, float (&z)[NT][4]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[nt][i] = zero[nt][i & 1];
+    const uint32_t at = st + sub * 16 * RB + chunk_at(lane & 15, KS == 1 && kInt8 ? 0 : lane >> 4);
+    if constexpr (kInt8) {
+      // A matrix of eight rows by 16 codes; four of them are two steps of 16 d.
+#pragma unroll
+      for (int s = 0; s < KS; s += 2) {
+        uint32_t x[4];
+        if constexpr (KS == 1)
+          ldmatrix2<false>(at, x);
+        else
+          ldmatrix4<false>(chunk_from(at, s), x);
+#pragma unroll
+        for (int w = 0; w < (KS == 1 ? 1 : 2); ++w) {
+          const uint32_t a[4] = {__byte_perm(x[2 * w], 0, 0x4140), __byte_perm(x[2 * w + 1], 0, 0x4140),
+                                 __byte_perm(x[2 * w], 0, 0x4342), __byte_perm(x[2 * w + 1], 0, 0x4342)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(z[nt], a, qf[nt][s + w][0], qf[nt][s + w][1]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        uint32_t a[4];
+        ldmatrix4<false>(chunk_from(at, 2 * s), a);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816(z[nt], a, qf[nt][s][0], qf[nt][s][1]);
+      }
+    }
+  }
+
+  // O^T += V^T P^T for one 16-key block.
+  __device__ __forceinline__ void values(uint32_t st, int sub, const uint32_t (&pb)[NT][2]) {
+    const uint32_t v = st + kArray + sub * 16 * RB;
+    if constexpr (kInt8) {
+      // Transposed as 16-bit pairs: lane (g, t) gets columns 2g, 2g + 1 of the keys 2t, 2t + 1.
+      const uint32_t at = v + chunk_at(lane & 15, MT == 1 ? 0 : lane >> 4);
+#pragma unroll
+      for (int j = 0; j < MT; j += 2) {
+        uint32_t x[4];
+        if constexpr (MT == 1)
+          ldmatrix2<true>(at, x);
+        else
+          ldmatrix4<true>(chunk_from(at, j), x);
+#pragma unroll
+        for (int w = 0; w < (MT == 1 ? 1 : 2); ++w) {
+          const uint32_t a[4] = {codes_to_half2<0x4240>(x[2 * w]), codes_to_half2<0x4341>(x[2 * w]),
+                                 codes_to_half2<0x4240>(x[2 * w + 1]), codes_to_half2<0x4341>(x[2 * w + 1])};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(o[j + w][nt], a, pb[nt][0], pb[nt][1]);
+        }
+      }
+    } else {
+      // Matrices in the order (keys 0-7, d 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15).
+      const uint32_t at = v + chunk_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        uint32_t a[4];
+        ldmatrix4<true>(chunk_from(at, 2 * j), a);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816(o[j][nt], a, pb[nt][0], pb[nt][1]);
+      }
+    }
+  }
+
+  // Softmax of a block's scores (z + lv in log2 units) and their products with V.
+  __device__ __forceinline__ void accumulate(uint32_t st, float (&z)[SUB][NT][4], const float (&rv)[SUB][2]) {
     bool grow = false;
     float top[NT][2];
 #pragma unroll
@@ -199,7 +306,7 @@ struct MmaCore {
       for (int q = 0; q < 2; ++q) {
         float x = -kInf;
 #pragma unroll
-        for (int b = 0; b < N; ++b) x = fmaxf(x, fmaxf(z[b][nt][q], z[b][nt][q + 2]));
+        for (int b = 0; b < SUB; ++b) x = fmaxf(x, fmaxf(z[b][nt][q], z[b][nt][q + 2]));
         top[nt][q] = x;
         grow |= x > m[nt][q] + 8.f;
       }
@@ -221,16 +328,18 @@ struct MmaCore {
           }
         }
     }
-    uint32_t pb[N][NT][2];
+    uint32_t pb[SUB][NT][2];
 #pragma unroll
-    for (int b = 0; b < N; ++b)
+    for (int nt = 0; nt < NT; ++nt) {
+      float ref[2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int q = 0; q < 2; ++q) ref[q] = m[nt][q] == -kInf ? 0.f : m[nt][q];  // a row that has seen nothing yet
+#pragma unroll
+      for (int b = 0; b < SUB; ++b) {
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float ref = m[nt][i & 1] == -kInf ? 0.f : m[nt][i & 1];  // a row that has seen nothing yet
-          e[i] = ex2(z[b][nt][i] - ref);
+          e[i] = ex2(z[b][nt][i] - ref[i & 1]);
           if constexpr (kInt8)
             l[nt][i & 1] = fmaf(e[i], rv[b][i >> 1], l[nt][i & 1]);
           else
@@ -239,62 +348,95 @@ struct MmaCore {
         pb[b][nt][0] = transpose8x8(pack_half2(e[0], e[1]));
         pb[b][nt][1] = transpose8x8(pack_half2(e[2], e[3]));
       }
+    }
 #pragma unroll
-    for (int b = 0; b < N; ++b) {
+    for (int b = 0; b < SUB; ++b) values(st, b, pb[b]);
+  }
+
+  // This lane's key of the stage: its field and scales.
+  struct Field {
+    float phi, psi, f, lv, rv;
+  };
+  __device__ __forceinline__ Field field_of(const DecodeParams& p, uint32_t st, bool ok) {
+    auto word = [&](int i) {
+      float x;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(st + 2 * kArray + (i * kKeys + lane) * 4) : "memory");
+      return x;
+    };
+    Field f{kInf, 0.f, 0.f, -kInf, 1.f};
+    if (ok) {
+      f.phi = word(0);
+      f.psi = word(1);
+      f.f = p.scale2;
+      f.lv = 0.f;
       if constexpr (kInt8) {
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          const uint32_t k0 = vf[b][0][w] ^ 0x80808080u, k1 = vf[b][1][w] ^ 0x80808080u;
-          const uint32_t k2 = vf[b][2][w] ^ 0x80808080u, k3 = vf[b][3][w] ^ 0x80808080u;
-#pragma unroll
-          for (int half = 0; half < (MT < 2 ? 1 : 2); ++half) {
-            const uint32_t x = half ? __byte_perm(k0, k1, 0x7362) : __byte_perm(k0, k1, 0x5140);
-            const uint32_t y = half ? __byte_perm(k2, k3, 0x7362) : __byte_perm(k2, k3, 0x5140);
-            const uint32_t a[4] = {codes_to_half2<0x4140>(x), codes_to_half2<0x4342>(x), codes_to_half2<0x4140>(y),
-                                   codes_to_half2<0x4342>(y)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816(o[2 * w + half][nt], a, pb[b][nt][0], pb[b][nt][1]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const uint32_t a[4] = {__byte_perm(vf[b][0][j], vf[b][1][j], 0x5410), __byte_perm(vf[b][0][j], vf[b][1][j], 0x7632),
-                                 __byte_perm(vf[b][2][j], vf[b][3][j], 0x5410), __byte_perm(vf[b][2][j], vf[b][3][j], 0x7632)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(o[j][nt], a, pb[b][nt][0], pb[b][nt][1]);
-        }
+        const float v = fmaxf(word(3), 0x1p-90f);
+        f.f *= word(2) * 0x1p24f;
+        f.lv = lg2(v);
+        f.rv = rcp_approx_f(v);
       }
     }
+    return f;
   }
 
   template <bool kPrefix>
   __device__ __forceinline__ void run(const DecodeParams& p, const Job& job) {
     const CacheView& c = p.c;
-    const int lane = threadIdx.x & 31;
-    // The first loads of the run go out before anything else.
-    int tile = job.t1 - 1;
-    int64_t base = -1, next = -1;
-    int lim = 0;
-    float phi = kInf, psi = 0.f, ks = 0.f, vs = 0.f;
-    if (tile >= job.t0) {
-      base = slot_of(c, job.table, job.h, tile * 32);
-      if (tile > job.t0) next = slot_of(c, job.table, job.h, tile * 32 - 32);
-      lim = base < 0 ? 0 : min(32, job.end - tile * 32);
-      load_k_step(c, base, 0, lim);
-      load_v_step(c, base, 0, lim);
-      if (lane < lim) {
-        phi = c.phi[base + lane];
-        psi = c.psi[base + lane];
-        if (kInt8) {
-          ks = c.ks[base + lane];
-          vs = c.vs[base + lane];
-        }
+    // The run's blocks from the latest to the earliest. First the table's entries that the start needs, all at once,
+    // with the queries; then all that they lead to: two dependent trips to memory instead of one for each use.
+    const int history = job.t1 - job.t0, total = history + (job.last ? 1 : 0);
+    int next = job.t1 - 1;  // next block to fetch
+    const int pid0 = history > 0 ? job.table[(next * kKeys) >> c.page_shift] : -1;
+    const int pid1 = history > 1 ? job.table[((next - 1) * kKeys) >> c.page_shift] : -1;
+    const int pid2 = kStages == 3 && history > 2 ? job.table[((next - 2) * kKeys) >> c.page_shift] : -1;
+    const int pid_new = !kPrefix && lane < job.n_new ? job.table[(job.end + lane) >> c.page_shift] : -1;
+    LaterMin later;
+    later.ids(c, job.table, job.t1 * kKeys, history > 0 ? job.end : 0);
+    load_q<kPrefix>(p, job);
+    int64_t base = -1;
+    auto fetch_block = [&](int i) {
+      const int lim = base < 0 ? 0 : min(kKeys, job.end - next * kKeys);
+      fetch(c, ring + (i % kStages) * kStage, base < 0 ? 0 : base, lim);
+      --next;
+    };
+    auto fetch_next = [&](int i) {
+      // Block i of the run into its stage; the place of the one after it, where that lies in another page, is looked
+      // up meanwhile.
+      fetch_block(i);
+      if (i + 1 < history) {
+        if (((next + 1) * kKeys & ((1 << c.page_shift) - 1)) != 0 && base >= 0)
+          base -= kKeys;
+        else
+          base = slot_of(c, job.table, job.h, next * kKeys);
+      }
+    };
+    if (history > 0) {
+      base = slot_in(c, pid0, job.h, next * kKeys);
+      fetch_block(0);
+    }
+    if (history > 0 || !job.last) copy_commit();  // else the newest tokens' place is not known yet
+    if constexpr (kStages == 3) {
+      if (history > 1) {
+        base = slot_in(c, pid1, job.h, next * kKeys);
+        fetch_block(1);
+      }
+      if (history > 1 || !job.last) copy_commit();
+      if (history > 2) base = slot_in(c, pid2, job.h, next * kKeys);
+    } else {
+      if (history > 1) base = slot_in(c, pid1, job.h, next * kKeys);
+    }
+    NewTokens nw{kInf, 0.f, kInf, -1, 0};
+    if constexpr (!kPrefix) nw = load_new(c, pid_new, job.h, job.end, job.n_new);
+    later.values(c, job.h);
+    sum_q();
+    nw.low = prefix_min(nw.phi);
+    if (job.last && history < kStages - 1) {
+      // Few blocks: the newest tokens' block and the empty groups after it.
+      for (int i = history; i < kStages - 1; ++i) {
+        if (i == history) fetch_new(c, ring + (i % kStages) * kStage, nw);
+        copy_commit();
       }
     }
-    load_q<kPrefix>(p, job);
-    NewTokens nw{kInf, 0.f, kInf, -1, 0};
-    if constexpr (!kPrefix) nw = load_new(c, job.table, job.h, job.end, job.n_new);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -312,116 +454,70 @@ struct MmaCore {
 #pragma unroll
         for (int j = 0; j < MT; ++j) o[j][nt][q] = o[j][nt][q + 2] = 0.f;
       }
-    if (tile >= job.t0) {
-      float mid = job.t1 * 32 < job.end ? later_min(c, job.table, job.h, job.t1 * 32, job.end) : kInf;
-      for (; tile >= job.t0; --tile) {
+    float mid = later.finish(c, job.table, job.h);
+    for (int i = 0; i < total; ++i) {
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      if (i + kStages - 1 < history)
+        fetch_next(i + kStages - 1);
+      else if (job.last && i + kStages - 1 == history)
+        fetch_new(c, ring + ((i + kStages - 1) % kStages) * kStage, nw);
+      copy_commit();
+      const uint32_t st = ring + (i % kStages) * kStage;
+      float z[SUB][NT][4], rv[SUB][2];
+#pragma unroll
+      for (int sub = 0; sub < SUB; ++sub) scores(st, sub, z[sub]);
+      if (i < history) {
+        const int tile = job.t1 - 1 - i;
+        const Field f = field_of(p, st, lane < kKeys && tile * kKeys + lane < job.end);
         float all;
-        const float suf = fminf(suffix_min(phi, all), mid);
+        const float suf = fminf(suffix_min(f.phi, all), mid);
         mid = fminf(mid, all);
-        const bool ok = lane < lim;
-        __syncwarp();
-        float lv = ok ? 0.f : -kInf;
-        if constexpr (kInt8) {
-          const float v = fmaxf(vs, 0x1p-90f);
-          if (ok) lv = lg2(v);
-          rvs[lane] = rcp_approx_f(v);
+        if (lane < kKeys) {
+          par[lane] = make_float4(fminf(suf - f.psi, 0.f), f.psi, f.f, f.lv);
+          if (kInt8) rvs[lane] = f.rv;
         }
-        par[lane] = make_float4(ok ? fminf(suf - psi, 0.f) : 0.f, psi, ok ? (kInt8 ? ks : 1.f) * p.scale2 : 0.f, lv);
         __syncwarp();
-        // The next tile's field and scales, and the page after it.
-        const int64_t here = base;
-        const int lim_here = lim;
-        base = next;
-        lim = tile > job.t0 && base >= 0 ? 32 : 0;
-        next = tile - 1 > job.t0 ? slot_of(c, job.table, job.h, tile * 32 - 64) : -1;
-        phi = kInf;
-        psi = ks = vs = 0.f;
-        if (lane < lim) {
-          phi = c.phi[base + lane];
-          psi = c.psi[base + lane];
-          if (kInt8) {
-            ks = c.ks[base + lane];
-            vs = c.vs[base + lane];
+#pragma unroll
+        for (int sub = 0; sub < SUB; ++sub)
+#pragma unroll
+          for (int key = 0; key < 2; ++key) {
+            const int at = sub * 16 + key * 8 + g;
+            const float4 x = par[at];
+            rv[sub][key] = kInt8 ? rvs[at] : 1.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                float& zz = z[sub][nt][2 * key + q];
+                zz = fmaf(zz, x.z, fmaf(job.bias, fminf(x.x, low[nt][q] - x.y), x.w));
+              }
           }
-        }
+      } else {
+        // The newest tokens among themselves: range minima pair by pair.
+        const Field f = field_of(p, st, lane < kKeys && nw.slot >= 0);
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-          float z[SUB][NT][4], rv[SUB][2];
+        for (int sub = 0; sub < SUB; ++sub)
 #pragma unroll
-          for (int sub = 0; sub < SUB; ++sub) scores(sub, z[sub]);
-          if (st + 1 < STEPS)
-            load_k_step(c, here, st + 1, lim_here);
-          else
-            load_k_step(c, base, 0, lim);
+          for (int key = 0; key < 2; ++key) {
+            const int j = sub * 16 + key * 8 + g;
+            const float ff = __shfl_sync(0xffffffffu, f.f, j & 31), lv = __shfl_sync(0xffffffffu, f.lv, j & 31);
+            rv[sub][key] = __shfl_sync(0xffffffffu, f.rv, j & 31);
 #pragma unroll
-          for (int sub = 0; sub < SUB; ++sub)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int key = 0; key < 2; ++key) {
-              const int at = (st * SUB + sub) * 16 + key * 8 + g;
-              const float4 x = par[at];
-              rv[sub][key] = kInt8 ? rvs[at] : 1.f;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                  const float b = fminf(x.x, low[nt][q] - x.y);
-                  float& zz = z[sub][nt][2 * key + q];
-                  zz = fmaf(zz, x.z, fmaf(job.bias, b, x.w));
-                }
-            }
-          accumulate<SUB>(z, rv);
-          if (st + 1 < STEPS)
-            load_v_step(c, here, st + 1, lim_here);
-          else
-            load_v_step(c, base, 0, lim);
-        }
+              for (int q = 0; q < 2; ++q) {
+                const int i_ = job.r0 + nt * 8 + 2 * t + q - job.lead;
+                const float b = new_pair(nw, j, i_);
+                float& zz = z[sub][nt][2 * key + q];
+                zz = j < job.n_new && j <= i_ ? fmaf(zz, ff, fmaf(job.bias, b, lv)) : -kInf;
+              }
+          }
       }
+      accumulate(st, z, rv);
+      __syncwarp();
     }
-    if constexpr (!kPrefix)
-      if (job.last) run_new(p, job, nw);
-  }
-
-  // The newest tokens among themselves: one block of up to 16 keys, whose range minima are taken pair by pair.
-  __device__ __forceinline__ void run_new(const DecodeParams& p, const Job& job, const NewTokens& nw) {
-    const CacheView& c = p.c;
-#pragma unroll
-    for (int key = 0; key < 2; ++key) {
-      const int64_t slot = __shfl_sync(0xffffffffu, nw.slot, key * 8 + g);
-      load_k(c, slot, 0, key, slot >= 0 ? 16 : 0);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t slot = __shfl_sync(0xffffffffu, nw.slot, (i >> 1) * 8 + 2 * t + (i & 1));
-      load_v(c, slot, 0, i, slot >= 0 ? 16 : 0);
-    }
-    float z[1][NT][4], rv[1][2];
-    scores(0, z[0]);
-#pragma unroll
-    for (int key = 0; key < 2; ++key) {
-      const int j = key * 8 + g;
-      const int64_t slot = __shfl_sync(0xffffffffu, nw.slot, j);
-      float f = p.scale2, lv = 0.f;
-      rv[0][key] = 1.f;
-      if constexpr (kInt8) {
-        if (slot >= 0) {
-          const float v = fmaxf(c.vs[slot], 0x1p-90f);
-          f *= c.ks[slot];
-          lv = lg2(v);
-          rv[0][key] = rcp_approx_f(v);
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int i = job.r0 + nt * 8 + 2 * t + q - job.lead;
-          const float b = new_pair(nw, j, i);
-          float& zz = z[0][nt][2 * key + q];
-          zz = slot >= 0 && j <= i ? fmaf(zz, f, fmaf(job.bias, b, lv)) : -kInf;
-        }
-    }
-    float (&zz)[1][NT][4] = z;
-    accumulate<1>(zz, rv);
+    copy_wait<0>();
   }
 
   __device__ __forceinline__ void store(float* sm, float* sl, float* sO, int rows) {
@@ -440,8 +536,9 @@ struct MmaCore {
           }
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
-            const int i = 2 * j, d = (i / VE * 8 + g) * VE + i % VE;
-            *reinterpret_cast<float2*>(sO + r * D + d) = make_float2(o[j][nt][q], o[j][nt][q + 2]);
+            float* at = sO + r * D + j * 16;
+            at[kInt8 ? 2 * g : g] = o[j][nt][q];
+            at[kInt8 ? 2 * g + 1 : g + 8] = o[j][nt][q + 2];
           }
         }
       }
@@ -449,28 +546,28 @@ struct MmaCore {
 };
 
 template <bool kInt8>
-cudaError_t launch_for(const DecodeParams& p, bool prefix, int splits, cudaStream_t s) {
+cudaError_t launch_for(const DecodeParams& p, bool prefix, cudaStream_t s) {
   // 16 rows at a time where there are more than 8, except at D = 256, whose accumulators leave no registers for them.
   const bool wide = (prefix ? p.B * p.n : p.n) > 8;
   switch (p.c.D) {
 #define FPA_CASE(D)                                                                            \
   case D:                                                                                      \
-    return wide ? launch_decode_core<MmaCore<D, kInt8, 2>>(p, prefix, splits, s)               \
-                : launch_decode_core<MmaCore<D, kInt8, 1>>(p, prefix, splits, s);
+    return wide ? launch_decode_core<MmaCore<D, kInt8, 2>>(p, prefix, s)               \
+                : launch_decode_core<MmaCore<D, kInt8, 1>>(p, prefix, s);
     FPA_CASE(16)
     FPA_CASE(32)
     FPA_CASE(64)
     FPA_CASE(128)
 #undef FPA_CASE
     default:
-      return launch_decode_core<MmaCore<256, kInt8, 1>>(p, prefix, splits, s);
+      return launch_decode_core<MmaCore<256, kInt8, 1>>(p, prefix, s);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, int splits, cudaStream_t s) {
-  return int8 ? launch_for<true>(p, prefix, splits, s) : launch_for<false>(p, prefix, splits, s);
+cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s) {
+  return int8 ? launch_for<true>(p, prefix, s) : launch_for<false>(p, prefix, s);
 }
 
 }  // namespace fpa

@@ -62,8 +62,8 @@ struct DecodeParams {
 };
 
 // Rows are handled by one CTA in groups of 8 or 16 (tensor cores) or 1, 4 or 8 (FFMA).
-cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, int splits, cudaStream_t s);
-cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, int splits, cudaStream_t s);
+cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s);
+cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s);
 cudaError_t launch_row_min(const DecodeParams& p, cudaStream_t s);
 
 int sm_count();  // fpa_tma.cu

@@ -18,32 +18,47 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import LaunchStats, _on_device, _stream
+from .ops import LaunchStats, _on_device
 
 MAX_NEW_TOKENS = 16
 _PAGE_SIZES = (32, 64, 128, 256)
 _HEAD_DIMS = (16, 32, 64, 128, 256)
 
 
-def _int32_on(name, x, device, shape=None):
-    if x.dtype != torch.int32 or x.device != device:
-        raise ValueError(f"{name} must be an int32 tensor on {device}")
-    if shape is not None and (x.shape != shape or not x.is_contiguous()):
+# The current stream's handle by device index, without building a Stream object (which costs as much as the launch).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _int32_on(name, x, index, shape):
+    if x.dtype != torch.int32 or x.get_device() != index:
+        raise ValueError(f"{name} must be an int32 tensor on cuda:{index}")
+    if x.shape != shape or not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous with shape {tuple(shape)}")
     return x.data_ptr()
 
 
-def _table_on(name, x, device, B):
-    if x.dtype != torch.int32 or x.device != device:
-        raise ValueError(f"{name} must be an int32 tensor on {device}")
+def _table_on(x, index, B):
+    if x.dtype != torch.int32 or x.get_device() != index:
+        raise ValueError(f"block_table must be an int32 tensor on cuda:{index}")
     if x.dim() != 2 or x.shape[0] != B or x.shape[1] < 1 or (x.stride(1) != 1 and x.shape[1] > 1):
-        raise ValueError(f"{name} must have shape (B, pages) with contiguous rows")
+        raise ValueError("block_table must have shape (B, pages) with contiguous rows")
     return x.data_ptr(), x.stride(0), x.shape[1]
 
 
-def _call(fn, args, device):
-    with _on_device(device):
-        _lib.check(fn(ctypes.byref(args), _stream(device)))
+def _call(fn, args, index):
+    if torch.cuda.current_device() == index:
+        rc = fn(ctypes.byref(args), _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(ctypes.byref(args), _raw_stream(index))
+    if rc:
+        _lib.check(rc)
+
+
+def _empty(shape, dtype, device):
+    B, H, n, D = shape
+    return torch.empty_strided(shape, (H * n * D, n * D, D, 1), dtype=dtype, device=device)
 
 
 class FPACache:
@@ -53,7 +68,8 @@ class FPACache:
     for pages that a sequence has filled).
 
     dtype: of k, v, q and o (float16 or float32). storage: None (as dtype) or torch.int8: scale = max|x| / 127 for each
-    token and head, code = round(127 x / max|x|), the value is code * scale."""
+    token and head (at least 2^-90), code = round(127 x / max|x|), the value is code * scale; the pool holds code + 128 as
+    uint8."""
 
     def __init__(self, n_pages, n_heads, head_dim, page_size=64, dtype=torch.float16, storage=None, device="cuda"):
         if dtype not in (torch.float16, torch.float32):
@@ -74,7 +90,8 @@ class FPACache:
         self.n_pages, self.n_heads, self.head_dim, self.page_size = n_pages, n_heads, head_dim, page_size
         self.dtype, self.storage, self.device = dtype, storage or dtype, device
         slots = (n_pages, n_heads, page_size)
-        self.k = torch.zeros(*slots, head_dim, dtype=self.storage, device=device)
+        self.k = torch.full((*slots, head_dim), 128, dtype=torch.uint8, device=device) if self.storage == torch.int8 else \
+            torch.zeros(*slots, head_dim, dtype=self.storage, device=device)
         self.v = torch.zeros_like(self.k)
         self.phi, self.psi = torch.zeros(slots, device=device), torch.zeros(slots, device=device)
         self.phi_min = torch.zeros(slots[:2], device=device)
@@ -88,7 +105,7 @@ class FPACache:
             n_pages, n_heads, page_size, head_dim,
             *(None if x is None else x.data_ptr() for x in (self.k, self.v, self.k_scale, self.v_scale, self.phi,
                                                             self.psi, self.phi_min, self._status)))
-        self._addr = ctypes.addressof(self._struct)
+        self._addr, self._index = ctypes.addressof(self._struct), device.index
 
     def append(self, k, v, phi, psi, block_table, start, counts=None):
         """Write the tokens k, v [B, H, n, D], phi, psi [B, H, n] (any strides) at positions start[b], start[b] + 1, ...
@@ -105,15 +122,15 @@ class FPACache:
             raise ValueError(f"phi and psi must have shape (B, {H}, n)")
         if phi.dtype != torch.float32 or psi.dtype != torch.float32:
             raise ValueError("phi and psi must be float32")
-        dev = self.device
-        if k.device != dev or v.device != dev or phi.device != dev or psi.device != dev:
-            raise ValueError(f"k, v, phi and psi must be on the cache's device {dev}")
+        dev = self._index
+        if k.get_device() != dev or v.get_device() != dev or phi.get_device() != dev or psi.get_device() != dev:
+            raise ValueError(f"k, v, phi and psi must be on the cache's device cuda:{dev}")
         if B == 0 or n == 0:
             return
         a = _lib.FpaAppendArgs()
         _lib.APPEND_PACKER.pack_into(
             a, 0, self._addr, B, n, k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), phi.data_ptr(), *phi.stride(),
-            psi.data_ptr(), *psi.stride(), *_table_on("block_table", block_table, dev, B),
+            psi.data_ptr(), *psi.stride(), *_table_on(block_table, dev, B),
             _int32_on("start", start, dev, (B,)), 0 if counts is None else _int32_on("counts", counts, dev, (B,)))
         _call(lib.fpa_cache_append, a, dev)
         LaunchStats.kernels += 1
@@ -122,15 +139,15 @@ class FPACache:
         """k, v [B, H, n, D] in the cache's dtype and phi, psi [B, H, n] at positions start[b] .. start[b] + n - 1 (from
         0 with start None); positions from lengths[b] on (or beyond the table) are zeros."""
         lib = _lib.load()
-        B, H, D, dev = block_table.shape[0], self.n_heads, self.head_dim, self.device
+        B, H, D, dev = block_table.shape[0], self.n_heads, self.head_dim, self._index
         if n < 0:
             raise ValueError("n must not be negative")
-        table = _table_on("block_table", block_table, dev, B)
+        table = _table_on(block_table, dev, B)
         start = 0 if start is None else _int32_on("start", start, dev, (B,))
         lengths = 0 if lengths is None else _int32_on("lengths", lengths, dev, (B,))
-        k = torch.empty((B, H, n, D), dtype=self.dtype, device=dev)
+        k = _empty((B, H, n, D), self.dtype, self.device)
         v = torch.empty_like(k)
-        phi = torch.empty((B, H, n), dtype=torch.float32, device=dev)
+        phi = torch.empty_strided((B, H, n), (H * n, n, 1), dtype=torch.float32, device=self.device)
         psi = torch.empty_like(phi)
         if B and n:
             a = _lib.FpaReadArgs()
@@ -145,7 +162,7 @@ class FPACache:
         length outside a block table (such entries are skipped, never touched)."""
         lib = _lib.load()
         with _on_device(self.device):
-            _lib.check(lib.fpa_workspace_status(ctypes.c_void_p(self._status.data_ptr()), _stream(self.device)))
+            _lib.check(lib.fpa_workspace_status(self._status.data_ptr(), _raw_stream(self._index)))
 
 
 def first_passage_decode(q, cache, block_table, lengths, beta, prefix_table=None, prefix_len=0):
@@ -157,16 +174,16 @@ def first_passage_decode(q, cache, block_table, lengths, beta, prefix_table=None
     token of every sequence, such as a system prompt; lengths do not count them, and they are read once for the whole
     batch. Equal to the last n rows of ``first_passage_attention`` over the whole sequence."""
     lib = _lib.load()
-    H, D, dev = cache.n_heads, cache.head_dim, cache.device
+    H, D, dev = cache.n_heads, cache.head_dim, cache._index
     if q.dim() != 4 or q.shape[1] != H or q.shape[3] != D:
         raise ValueError(f"q must have shape (B, {H}, n, {D})")
     B, _, n, _ = q.shape
     if not 1 <= n <= MAX_NEW_TOKENS:
         raise ValueError(f"between 1 and {MAX_NEW_TOKENS} new tokens per call")
-    if q.dtype != cache.dtype or q.device != dev:
-        raise ValueError(f"q must be {cache.dtype} on {dev}")
-    if beta.shape != (H,) or beta.dtype != torch.float32 or beta.device != dev or not beta.is_contiguous():
-        raise ValueError(f"beta must be a contiguous float32 tensor of shape ({H},) on {dev}")
+    if q.dtype != cache.dtype or q.get_device() != dev:
+        raise ValueError(f"q must be {cache.dtype} on {cache.device}")
+    if beta.shape != (H,) or beta.dtype != torch.float32 or beta.get_device() != dev or not beta.is_contiguous():
+        raise ValueError(f"beta must be a contiguous float32 tensor of shape ({H},) on {cache.device}")
     pages, ptable = 0, 0
     if prefix_len < 0 or (prefix_len > 0 and prefix_table is None):
         raise ValueError("prefix_len must not be negative, and needs a prefix_table")
@@ -175,21 +192,21 @@ def first_passage_decode(q, cache, block_table, lengths, beta, prefix_table=None
         ptable = _int32_on("prefix_table", prefix_table, dev, (pages,))
         if pages * cache.page_size < prefix_len:
             raise ValueError("the prefix is longer than the pages of its table")
-    o = torch.empty((B, H, n, D), dtype=q.dtype, device=dev)
+    o = _empty((B, H, n, D), q.dtype, cache.device)
     if B == 0:
         return o
-    table = _table_on("block_table", block_table, dev, B)
+    table = _table_on(block_table, dev, B)
     lengths = _int32_on("lengths", lengths, dev, (B,))
     ws, ws_ptr, nbytes = None, 0, 0
-    with _on_device(dev):
-        if prefix_len > 0:
-            nbytes = lib.fpa_decode_workspace_bytes(ctypes.byref(cache._struct), B, n, prefix_len)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            ws_ptr = ws.data_ptr()
-        a = _lib.FpaDecodeArgs()
-        _lib.DECODE_PACKER.pack_into(a, 0, cache._addr, B, n, q.data_ptr(), *q.stride(), o.data_ptr(), *o.stride(),
-                                     beta.data_ptr(), *table, lengths, ptable, pages, prefix_len, ws_ptr, nbytes, 0)
-        _lib.check(lib.fpa_decode(ctypes.byref(a), _stream(dev)))
+    if prefix_len > 0:
+        with _on_device(cache.device):
+            nbytes = lib.fpa_decode_workspace_bytes(cache._struct, B, n, prefix_len)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device)
+        ws_ptr = ws.data_ptr()
+    a = _lib.FpaDecodeArgs()
+    _lib.DECODE_PACKER.pack_into(a, 0, cache._addr, B, n, q.data_ptr(), *q.stride(), o.data_ptr(), *o.stride(),
+                                 beta.data_ptr(), *table, lengths, ptable, pages, prefix_len, ws_ptr, nbytes, 0)
+    _call(lib.fpa_decode, a, dev)
     LaunchStats.kernels += a.kernels_launched
     return o
 
@@ -219,13 +236,14 @@ def verify_draft(p, q, draft, u, noise, draft_lens=None):
         raise ValueError("noise must be a float32 tensor of shape (B, V)")
     if V < 1:
         raise ValueError("the vocabulary must not be empty")
-    dev = p.device
-    if not p.is_cuda or any(x.device != dev for x in (q, draft, u, noise)):
+    dev = p.get_device()
+    if dev < 0 or q.get_device() != dev or draft.get_device() != dev or u.get_device() != dev or noise.get_device() != dev:
         raise ValueError("p, q, draft, u and noise must be on one CUDA device")
-    p, q, noise = (x if x.stride(-1) == 1 else x.contiguous() for x in (p, q, noise))
+    if p.stride(2) != 1 or q.stride(2) != 1 or noise.stride(1) != 1:
+        p, q, noise = (x if x.stride(-1) == 1 else x.contiguous() for x in (p, q, noise))
     lens = 0 if draft_lens is None else _int32_on("draft_lens", draft_lens, dev, (B,))
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    tokens = torch.empty((B, n + 1), dtype=torch.int64, device=dev)
+    accepted = torch.empty_strided((B,), (1,), dtype=torch.int32, device=p.device)
+    tokens = torch.empty_strided((B, n + 1), (n + 1, 1), dtype=torch.int64, device=p.device)
     if B == 0:
         return accepted, tokens
     a = _lib.FpaVerifyArgs()

@@ -129,7 +129,8 @@ enum FpaStorage { FPA_STORE_F16 = 0, FPA_STORE_F32 = 1, FPA_STORE_I8 = 2 };
 
 typedef struct FpaCache {
   int32_t dtype;            /* FpaDtype of k, v as handed in and out, and of q and o */
-  int32_t storage;          /* FpaStorage: that type, or int8 codes with a float32 scale per token and head */
+  int32_t storage;          /* FpaStorage: that type, or int8 codes (stored with 128 added) and a float32 scale
+                               per token and head */
   int32_t n_pages, H;
   int32_t page_size;        /* 32, 64, 128 or 256 */
   int32_t D;                /* 16, 32, 64, 128 or 256 */

@@ -57,10 +57,10 @@ def i32(x):
 
 
 def poison(cache):
-    """Everything a sequence has not written is NaN (127 in codes)."""
+    """Everything a sequence has not written is NaN (255 in the codes' bytes)."""
     for x in (cache.k, cache.v, cache.phi, cache.psi, cache.phi_min, cache.k_scale, cache.v_scale):
         if x is not None:
-            x.fill_(127 if x.dtype == I8 else float("nan"))
+            x.fill_(255 if x.dtype == torch.uint8 else float("nan"))
 
 
 def fill(cache, table, lens, k, v, phi, psi):
@@ -120,7 +120,7 @@ def test_append_and_read(dtype, storage, D, page):
             assert torch.equal(cache.phi_min[table[b, i]].cpu(), want), (b, i)
     if storage == I8:
         codes, scale, _ = quantise(k[0, :, :page])
-        assert torch.equal(cache.k[table[0, 0]].cpu(), codes)
+        assert torch.equal(cache.k[table[0, 0]].cpu().int() - 128, codes.int())
         assert torch.equal(cache.k_scale[table[0, 0]].cpu(), scale)
 
 
@@ -141,7 +141,7 @@ def test_append_odd_layouts():
     shared.append(k[:, :1].cuda().expand(B, H, n, D), v.cuda(), phi.cuda(), psi.cuda(), table, i32([0, 0]))
     for name in ("k", "v", "k_scale", "v_scale", "phi", "psi", "phi_min"):
         assert torch.equal(getattr(got, name), getattr(want, name)), name
-    assert torch.equal(shared.k[table[1, 0], 1, :n].cpu(), quantise(k[1, 0])[0])
+    assert torch.equal(shared.k[table[1, 0], 1, :n].cpu().int() - 128, quantise(k[1, 0])[0].int())
 
 
 def test_append_takes_back_refused_tokens():
