@@ -12,16 +12,21 @@ int invalid(const char* msg) {
   return FPA_ERR_INVALID_ARGUMENT;
 }
 
-// Parts of the prefix: enough CTAs for four per SM, at least two 32-key tiles for each of their four warps.
-int prefix_parts(int64_t units, int prefix_len) {
-  const int64_t most = (int64_t(prefix_len) + 255) / 256;
-  const int64_t want = (4 * sm_count() + units - 1) / units;
-  return int(want < 1 ? 1 : want > most ? most : want);
+// The prefix pass runs on tcgen05 for fp16 queries with D = 64 or 128 and more than 16 rows in the batch; 16 rows or
+// fewer fit one pass of the mma.sync kernel over the prefix.
+bool prefix_on_tc(const FpaCache& c, int64_t rows) {
+  return c.dtype == FPA_DTYPE_F16 && (c.D == 64 || c.D == 128) && rows > 16;
 }
 
+// Parts of the prefix (CTAs that share a row group's or row tile's prefix). tcgen05: one CTA on every SM, two 128-key
+// tiles each at least. Otherwise about four CTAs for an SM, two 32-key blocks for each of their four warps at least.
 int prefix_chunks(const FpaCache& c, int B, int n, int prefix_len) {
   const int64_t R = int64_t(B) * n;
-  return prefix_parts((R + 15) / 16 * c.H, prefix_len);
+  const bool tc = prefix_on_tc(c, R);
+  const int64_t most = (int64_t(prefix_len) + 255) / 256;
+  const int64_t units = (tc ? prefix_tc_row_tiles(R) : (R + 15) / 16) * c.H;
+  const int64_t want = tc ? sm_count() / units : (4 * sm_count() + units - 1) / units;
+  return int(want < 1 ? 1 : want > most ? most : want);
 }
 
 size_t workspace_bytes(const FpaCache& c, int B, int n, int prefix_len, size_t* ml, size_t* o) {
@@ -97,7 +102,7 @@ extern "C" FPA_API int fpa_decode(FpaDecodeArgs* a, void* stream) {
     e = launch_row_min(p, s);
     if (e == cudaSuccess) {
       prof_mark(s, "decode_prefix");
-      e = run(p, i8, true, s);
+      e = prefix_on_tc(c, int64_t(p.B) * p.n) ? launch_prefix_tc(p, i8, s) : run(p, i8, true, s);
     }
     if (e != cudaSuccess) {
       set_last_error(std::string("fpa_decode, prefix: ") + cudaGetErrorString(e));

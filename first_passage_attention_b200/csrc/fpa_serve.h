@@ -64,6 +64,9 @@ struct DecodeParams {
 // Rows are handled by one CTA in groups of 8 or 16 (tensor cores) or 1, 4 or 8 (FFMA).
 cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s);
 cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s);
+// The prefix on tcgen05: fp16 queries, D = 64 or 128. p.chunks: CTAs that share a row tile's prefix.
+int prefix_tc_row_tiles(int64_t rows);
+cudaError_t launch_prefix_tc(const DecodeParams& p, bool int8, cudaStream_t s);
 cudaError_t launch_row_min(const DecodeParams& p, cudaStream_t s);
 
 int sm_count();  // fpa_tma.cu

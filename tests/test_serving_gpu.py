@@ -68,11 +68,25 @@ def fill(cache, table, lens, k, v, phi, psi):
 
 
 def expected(q, k, v, phi, psi, beta, n, storage):
-    """The oracle's rows T - n .. T - 1 of one sequence ([H, T, ...] tensors), on the values that the cache holds."""
+    """Rows T - n .. T - 1 of one sequence ([H, T, ...] tensors) in float64, on the values that the cache holds."""
     if storage == I8:
         k, v = quantise(k)[2], quantise(v)[2]
-    a = [x.double().numpy()[None] for x in (q, k, v, phi, psi)]
-    return torch.from_numpy(O.forward(*a, beta.double().numpy())[0][0][:, -n:])
+    q, k, v, phi, psi, beta = (x.double().cuda() for x in (q, k, v, phi, psi, beta))
+    T, out = k.shape[1], []
+    for t in range(T - n, T):
+        least = phi[:, 1:t + 1].flip(-1).cummin(-1).values.flip(-1)  # min over s < u <= t, for s < t
+        z = (k[:, :t + 1] @ q[:, t, :, None])[..., 0] / q.shape[-1] ** 0.5
+        z[:, :t] += beta[:, None] * (least - psi[:, :t]).clamp(max=0)
+        out.append((z.softmax(-1)[:, None] @ v[:, :t + 1])[:, 0])
+    return torch.stack(out, 1).cpu()
+
+
+def test_expected_rows_are_the_oracles():
+    q, k, v, phi, psi = sequence(1, 2, 70, 32, F32, seed=20)
+    beta = torch.tensor([0.7, -0.4])
+    want = O.forward(*(x.double().numpy() for x in (q, k, v, phi, psi)), beta.double().numpy())[0][0][:, -9:]
+    got = expected(q[0], k[0], v[0], phi[0], psi[0], beta, 9, None)
+    assert (got - torch.from_numpy(want)).abs().max().item() <= 1e-12
 
 
 def assert_close(got, want, vmax, dtype, what=""):
@@ -256,6 +270,22 @@ def test_prefix(dtype, storage, D, n, P):
 @pytest.mark.parametrize("storage", [None, I8])
 def test_prefix_many_rows(B, n, storage):
     run_decode([(7 * b) % 90 for b in range(B)], n, 1, 64, 32, F16, storage, seed=B, P=300)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("storage", [None, I8])
+@pytest.mark.parametrize("B,n,P,page", [(17, 1, 1, 32), (8, 4, 128, 64), (11, 3, 257, 128), (16, 4, 640, 256), (13, 5, 1000, 32),
+                                        (40, 3, 129, 64), (43, 3, 2100, 128), (9, 15, 127, 32)])
+def test_prefix_on_the_tensor_cores(D, storage, B, n, P, page):
+    """17 to 135 rows: a quarter, half or all of the 128 lanes, and a second row tile; prefixes around tile ends."""
+    run_decode([(11 * b) % 50 for b in range(B)], n, 2, D, page, F16, storage, seed=B + P, P=P)
+
+
+def test_prefix_rows_far_apart():
+    """Rows whose scores differ by thousands beside ordinary ones, and a falling field: maxima that grow late."""
+    B, n, D, P = 30, 2, 64, 700
+    for beta, walk in ((4.0, 20.0), (-0.5, 3.0)):
+        run_decode([(5 * b) % 40 for b in range(B)], n, 2, D, 64, F16, I8, seed=17, P=P, beta=torch.full((2,), beta), walk=walk)
 
 
 def test_prefix_equals_whole_sequences():
