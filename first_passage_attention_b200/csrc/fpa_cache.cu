@@ -311,8 +311,10 @@ int check_cache(const FpaCache* c) {
     return invalid("the head dimension must be 16, 32, 64, 128 or 256");
   if (!c->k || !c->v || !c->phi || !c->psi || !c->phi_min || !c->status) return invalid("null cache pointer");
   if (c->storage == FPA_STORE_I8 && (!c->k_scale || !c->v_scale)) return invalid("null cache scale pointer");
-  if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
-    return invalid("the cache's k and v must be 16-byte aligned");
+  const void* arrays[] = {c->k, c->v, c->phi, c->psi, c->storage == FPA_STORE_I8 ? c->k_scale : nullptr,
+                          c->storage == FPA_STORE_I8 ? c->v_scale : nullptr};
+  for (const void* a : arrays)
+    if (reinterpret_cast<uintptr_t>(a) % 16) return invalid("the cache's arrays must be 16-byte aligned");
   return FPA_OK;
 }
 

@@ -2,19 +2,23 @@
 //
 // The rows (b, i) of all sequences, up to 128 at a time, meet every key of the prefix once: S = Q K^T and O += P V with
 // 128-key tiles, one CTA on an SM for a part of the prefix, which it walks from the latest tile to the earliest (the
-// mathematics is in fpa_decode.cuh). With R rows there are R flops a byte in fp16 and 2 R in int8, so up to about 128
-// rows the prefix's bytes bound it and beyond that the softmax's instructions do, about 7 for a (row, key) pair. Against
-// that, two softmax groups of 128 threads (a thread is a row is a TMEM lane) take alternate tiles, each with its own S,
-// running maximum, sum and O in TMEM, and their states join at the end. Where the rows fill half or a quarter of the
-// 128 lanes, they stand there twice or four times, and each copy takes its half or quarter of the tile's keys (its P
-// is zero for the others), so that no warp idles; the copies' states join like the groups'.
+// mathematics is in fpa_decode.cuh). With R rows there are R flops a byte in fp16 and 2 R in int8, so for few rows the
+// prefix's bytes bound it; at 128 rows and D = 128 a tile takes 1024 cycles of MMAs, as many of exponentials, and as
+// many to bring its 64 KB to the SM. Where the rows fill half or a quarter of the 128 lanes, they stand there twice or
+// four times, and each copy takes its half or quarter of the tile's keys (its P stays zero for the others), so that no
+// warp idles; the copies' softmax states join at the end.
 //
-// Warps 0-3 and 4-7: softmax groups. Warps 8-11: K and V into the ring of 128-byte-swizzled tiles; fp16 by cp.async
-// directly, int8 by cp.async into a raw ring that each thread reads back itself, converts to fp16 (exact) and stores.
-// Plain loads rather than TMA, because the last page's slots past the prefix must come out as zeros whatever they
-// hold, and because codes have to be converted on the way. Warp 12: the MMAs. Warp 13: per tile the keys' a, psi and
-// scales, with the running minimum of phi. Every wait is bounded.
+// Warps 0-3 and 4-7: two softmax groups; a thread is a row (a TMEM lane). Group g takes keys 64 g .. 64 g + 63 of every
+// tile, with its own running maximum, sum and O, so the groups never wait for each other and one's exponentials run
+// beside the other's products and minima; their states join at the end. Each group's S is double-buffered (P overwrites
+// the buffer it came from), so a tile's S is ready when its turn comes. Warps 8-11 and 12-15: K and V into the ring of 128-byte-swizzled tiles; fp16
+// by cp.async directly, int8 by cp.async into a raw ring that each thread reads back itself, converts to fp16 (exact)
+// and stores. Plain loads rather than TMA, because the last page's slots past the prefix must come out as zeros
+// whatever they hold, and because codes have to be converted on the way. Warp 16: the MMAs. Warps 17 and 18: the keys'
+// field and scales, alternate tiles. Every wait is bounded.
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "fpa_decode.cuh"
 #include "fpa_sm100.cuh"
@@ -25,32 +29,33 @@ namespace {
 using namespace sm100;
 
 constexpr int kTile = 128;
-constexpr int kPrefixThreads = 512;
-constexpr int kLoaders = 128;
+constexpr int kPrefixThreads = 640;
+constexpr int kLoaders = 128;   // of K, and as many of V
+constexpr int kWarpMma = 16, kWarpField = 17;
 constexpr int kParStages = 4;
 
 template <int D, bool kInt8>
 struct PrefixCfg {
   static constexpr int BOXB = kTile * 128;                // a tile's 64 columns
   static constexpr int TILEB = D / 64 * BOXB;             // K or V of a tile in fp16
-  static constexpr int SLOTS = kInt8 ? (D == 64 ? 6 : 4) : (D == 64 ? 8 : 5);
+  static constexpr int SLOTS = kInt8 ? (D == 64 ? 6 : 3) : (D == 64 ? 8 : 5);
   static constexpr int RAWB = kInt8 ? kTile * D : 0;      // K or V of a tile in codes
-  static constexpr int RAWS = kInt8 ? (D == 64 ? 4 : 3) : 0;
-  static constexpr int PARF = kInt8 ? 10 : 6;             // floats of a pair of keys
+  static constexpr int RAWS = kInt8 ? (D == 64 ? 3 : 2) : 0;  // of K, and as many of V
+  static constexpr int PARF = kInt8 ? 8 : 4;              // floats of a pair of keys
   static constexpr int PARB = kTile / 2 * PARF * 4;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_RING = OFF_Q + TILEB;
   static constexpr int OFF_RAW = OFF_RING + SLOTS * TILEB;
-  static constexpr int OFF_PAR = OFF_RAW + RAWS * RAWB;
-  static constexpr int OFF_ML = OFF_PAR + kParStages * PARB;  // [2][256] maxima and sums of the states
-  static constexpr int OFF_BAR = OFF_ML + 2 * 256 * 4;
-  static constexpr int NBAR = 2 * SLOTS + 2 * kParStages + 2 + 2 + 2;
+  static constexpr int OFF_PAR = OFF_RAW + 2 * RAWS * RAWB;
+  static constexpr int OFF_ML = OFF_PAR + kParStages * PARB;  // the states' maxima and sums [2][256]
+  static constexpr int OFF_BAR = OFF_ML + 512 * 4;
+  static constexpr int NBAR = 2 * SLOTS + 2 * kParStages + 10;
   static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
-  static constexpr int COL_S = 0, COL_O = 2 * kTile;      // of group g: + 128 g, + D g; P over the first half of S
+  static constexpr int COL_S = 0, COL_O = 2 * kTile;  // S of tile k: + 128 (k & 1), of group g: + 64 g; O: + D g
   static constexpr uint32_t IDESC_S = idesc_f16(kTile, kTile, 0);
   static constexpr uint32_t IDESC_O = idesc_f16(kTile, D, 1);
   static_assert(SMEM <= 227 * 1024, "shared memory");
-  static_assert(256 * (D + 1) * 4 <= SLOTS * TILEB + RAWS * RAWB, "the states join in the ring's place");
+  static_assert(256 * (D + 4) * 4 <= SLOTS * TILEB + 2 * RAWS * RAWB, "the states join in the ring's place");
 };
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -98,7 +103,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   uint64_t* par_empty = par_full + kParStages;
   uint64_t* s_full = par_empty + kParStages;
   uint64_t* p_full = s_full + 2;
-  uint64_t* q_full = p_full + 2;
+  uint64_t* o_ready = p_full + 4;
+  uint64_t* q_full = o_ready + 2;
   uint64_t* o_done = q_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -119,17 +125,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     }
     for (int i = 0; i < kParStages; ++i) {
       mbar_init(par_full + i, 32);
-      mbar_init(par_empty + i, 128);
+      mbar_init(par_empty + i, 256);
     }
-    for (int g = 0; g < 2; ++g) {
-      mbar_init(s_full + g, 1);
-      mbar_init(p_full + g, 128);
+    // P of group g, tile k: barrier 2 g + (k & 1). A warp can be a tile ahead of another of its group, but not two: S of
+    // tile k + 2 follows P V of tile k, which needs every warp's P.
+    for (int i = 0; i < 4; ++i) mbar_init(p_full + i, 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(o_ready + i, 1);
     }
     mbar_init(q_full, 256);
     mbar_init(o_done, 1);
     fence_mbar_init();
   }
-  if (warp == 12) tmem_alloc(tmem_slot, 512);
+  if (warp == kWarpMma) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -137,91 +146,132 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   // The launch before this one (row_min) has waited for everything earlier, so the cache and the queries can be read
   // at once; only the softmax warps wait, for the rows' minima.
 
-  // Registers: 128 a thread at launch; 184 for the softmax warpgroups, 72 for the others.
+  // Registers: 96 a thread at launch (61440 in all); 136 for the two softmax warpgroups, 64 for the other three (59392).
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
-    if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;" ::: "memory");
+    if (warp < kWarpMma) {
       // ------------------------------------------------------------------------------------------- K and V ----
-      const int tid = threadIdx.x - 256;
+      const int kv = (warp - 8) >> 2, tid = threadIdx.x - 256 - kv * kLoaders;  // K or V
       constexpr int kRowB = kInt8 ? D : 2 * D, CPR = kRowB / 16, kPer = kTile * CPR / kLoaders;
-      const int units = 2 * nt;  // K then V of each tile
-      int64_t base[4];           // pool index of each 32-key quarter of the current tile, or -1
-      // Unit u's chunks of this thread: chunk i is row (i 128 + tid) / CPR, so 128 / CPR rows apart.
-      auto copy_unit = [&](int u, uint32_t dst_base) {
-        const int tile = t1 - 1 - (u >> 1);
-        if ((u & 1) == 0) {
+      const char* pool = static_cast<const char*>(kv ? c.v : c.k);
+      // A thread's chunks lie kRows rows apart (a multiple of 8), in kQuarters of the tile's four 32-key quarters, each
+      // of which lies in one page: all four where kRows <= 32, else every other one.
+      constexpr int kRows = kLoaders / CPR, kQuarters = kRows <= 32 ? 4 : 2;
+      const int row0 = tid / CPR, ch = tid % CPR;
+      int64_t base[kQuarters];   // pool index of the quarters of the current tile, or -1
+      int pid[kQuarters];        // the next tile's table entries, looked up a tile ahead
+      bool whole = false;        // every key of the current tile exists
+      auto quarter = [&](int j) { return kRows <= 32 ? j : 2 * j + (row0 >> 5); };
+      auto chunk_quarter = [](int i) { return kRows <= 32 ? (i * kRows) >> 5 : i; };
+      constexpr int kInQuarter = kRows <= 32 ? kRows : 0;  // chunk i's row within its quarter: (i kInQuarter) & 31 + row0 & 31
+      auto look_up = [&](int tile) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int pos = tile * kTile + q * 32;
-            base[q] = pos < p.prefix_len ? slot_of(c, p.prefix_table, h, pos) : -1;
-          }
-        }
-        const char* src = static_cast<const char*>((u & 1) ? c.v : c.k);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int idx = i * kLoaders + tid, row = idx / CPR, ch = idx % CPR;
-          const int64_t b0 = base[(i * (kLoaders / CPR)) >> 5];  // rows of one i stay within 32 keys
-          const bool ok = b0 >= 0 && tile * kTile + row < p.prefix_len;
-          const char* from = src + ((b0 < 0 ? 0 : b0) + (row & 31)) * kRowB + ch * 16;
-          cp16(dst_base + (kInt8 ? uint32_t(idx * 16) : tile_chunk(row, ch)), from, ok);
+        for (int j = 0; j < kQuarters; ++j) {
+          const int pos = tile * kTile + quarter(j) * 32;
+          pid[j] = tile >= 0 && pos < p.prefix_len ? p.prefix_table[pos >> c.page_shift] : 0;
         }
       };
+      look_up(t1 - 1);
+      // Tile k's chunks of this thread to dst, `step` bytes apart. Tiles are taken in order.
+      auto copy_tile = [&](int k, uint32_t dst, auto step) {
+        const int tile = t1 - 1 - k;
+        whole = tile * kTile + kTile <= p.prefix_len;
+#pragma unroll
+        for (int j = 0; j < kQuarters; ++j) {
+          const int pos = tile * kTile + quarter(j) * 32;
+          base[j] = pos < p.prefix_len ? slot_in(c, pid[j], h, pos) : -1;
+          whole = whole && base[j] >= 0;
+        }
+        look_up(tile - 1);
+        const char* src = pool + (row0 & 31) * kRowB + ch * 16;
+        if (whole) {
+          const char* from[kQuarters];
+#pragma unroll
+          for (int j = 0; j < kQuarters; ++j) from[j] = src + base[j] * kRowB;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i)
+            cp16(dst + i * step, from[chunk_quarter(i)] + ((i * kInQuarter) & 31) * kRowB, true);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int64_t b0 = base[chunk_quarter(i)];
+            const bool ok = b0 >= 0 && tile * kTile + i * kRows + row0 < p.prefix_len;
+            cp16(dst + i * step, src + ((b0 < 0 ? 0 : b0) + ((i * kInQuarter) & 31)) * kRowB, ok);
+          }
+        }
+      };
+      // K of tile k is unit 2 k of the ring, V unit 2 k + 1.
       const uint32_t ring = smem_u32(smem + C::OFF_RING);
       bool ok = true;
       if constexpr (kInt8) {
-        const uint32_t raw = smem_u32(smem + C::OFF_RAW);
+        const uint32_t raw = smem_u32(smem + C::OFF_RAW) + kv * (C::RAWS * C::RAWB) + tid * 16;
+        constexpr std::integral_constant<uint32_t, kLoaders * 16> step{};
 #pragma unroll
-        for (int u = 0; u < C::RAWS - 1; ++u) {
-          if (u < units) copy_unit(u, raw + u * C::RAWB);
+        for (int k = 0; k < C::RAWS - 1; ++k) {
+          if (k < nt) copy_tile(k, raw + k * C::RAWB, step);
           cp_commit();
         }
-        for (int u = 0; u < units; ++u) {
-          const int un = u + C::RAWS - 1;
-          if (un < units) copy_unit(un, raw + (un % C::RAWS) * C::RAWB);
+        for (int k = 0; k < nt; ++k) {
+          const int kn = k + C::RAWS - 1;
+          if (kn < nt) copy_tile(kn, raw + (kn % C::RAWS) * C::RAWB, step);
           cp_commit();
           cp_wait<C::RAWS - 1>();
-          const int slot = u % C::SLOTS;
+          const int u = 2 * k + kv, slot = u % C::SLOTS;
           if (u >= C::SLOTS) ok = mbar_wait(empty + slot, ((u / C::SLOTS) - 1) & 1, c.status, 71);
           if (!ok) break;
-          const uint32_t from = raw + (u % C::RAWS) * C::RAWB, to = ring + slot * C::TILEB;
+          const uint32_t from = raw + (k % C::RAWS) * C::RAWB, to = ring + slot * C::TILEB;
+          const uint32_t to_a = to + tile_chunk(row0, 2 * ch), to_b = to + tile_chunk(row0, 2 * ch + 1);
           // Slots past the prefix hold zero bytes, which would be code -128: they are zero in fp16 too.
-          const int tile = t1 - 1 - (u >> 1);
+          const int live = p.prefix_len - (t1 - 1 - k) * kTile - row0;
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
-            const int idx = i * kLoaders + tid, row = idx / CPR, ch = idx % CPR;
-            const uint4 w = ld_shared16(from + idx * 16);
-            const bool live = tile * kTile + row < p.prefix_len;
-            uint4 a = make_uint4(code_pair<0x4140>(w.x), code_pair<0x4342>(w.x), code_pair<0x4140>(w.y), code_pair<0x4342>(w.y));
-            uint4 b = make_uint4(code_pair<0x4140>(w.z), code_pair<0x4342>(w.z), code_pair<0x4140>(w.w), code_pair<0x4342>(w.w));
-            if (!live) a = b = make_uint4(0, 0, 0, 0);
-            st_shared16(to + tile_chunk(row, 2 * ch), a);
-            st_shared16(to + tile_chunk(row, 2 * ch + 1), b);
+            uint4 w = ld_shared16(from + i * kLoaders * 16);
+            if (i * kRows >= live) w = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            st_shared16(to_a + i * kRows * 128, make_uint4(code_pair<0x4140>(w.x), code_pair<0x4342>(w.x),
+                                                           code_pair<0x4140>(w.y), code_pair<0x4342>(w.y)));
+            st_shared16(to_b + i * kRows * 128, make_uint4(code_pair<0x4140>(w.z), code_pair<0x4342>(w.z),
+                                                           code_pair<0x4140>(w.w), code_pair<0x4342>(w.w)));
           }
           fence_async_proxy();
           mbar_arrive(full + slot);
         }
       } else {
-        // Up to kAhead units in flight beyond the one that is handed over.
-        constexpr int kAhead = C::SLOTS - 2;
-        int sent = 0;
-        for (int u = 0; u < units + kAhead && ok; ++u) {
-          if (u < units) {
-            const int slot = u % C::SLOTS;
-            if (u >= C::SLOTS) ok = mbar_wait(empty + slot, ((u / C::SLOTS) - 1) & 1, c.status, 72);
+        // A tile is handed over when kAhead younger ones are on their way, or when the ring is full, so that there is
+        // nothing to fetch anyhow.
+        constexpr int kAhead = C::SLOTS / 2 - 1;
+        int handed = 0;
+        auto hand_over = [&]() {
+          fence_async_proxy();
+          mbar_arrive(full + (2 * handed + kv) % C::SLOTS);
+          ++handed;
+        };
+        for (int k = 0; k < nt; ++k) {
+          const int u = 2 * k + kv, slot = u % C::SLOTS;
+          if (u >= C::SLOTS) {
+            const uint32_t parity = ((u / C::SLOTS) - 1) & 1;
+            while (handed < k && !__all_sync(0xffffffffu, mbar_test_wait(empty + slot, parity))) {
+              if (k - handed > 1 && kAhead > 1)
+                cp_wait<1>();  // all but the youngest
+              else
+                cp_wait<0>();
+              hand_over();
+            }
+            ok = mbar_wait(empty + slot, parity, c.status, 72);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            copy_unit(u, ring + slot * C::TILEB);
           }
+          copy_tile(k, ring + slot * C::TILEB + tile_chunk(row0, ch), std::integral_constant<uint32_t, kRows * 128>{});
           cp_commit();
-          if (u >= kAhead) {
+          if (k - handed >= kAhead) {
             cp_wait<kAhead>();
-            fence_async_proxy();
-            mbar_arrive(full + sent % C::SLOTS);
-            ++sent;
+            hand_over();
           }
         }
+        cp_wait<0>();
+        while (ok && handed < nt) hand_over();
       }
       cp_wait<0>();
-    } else if (warp == 12) {
+    } else if (warp == kWarpMma) {
       // ------------------------------------------------------------------------------------------------ MMA ----
       const bool leader = elect_one();
       constexpr uint32_t HI = desc_hi(8 * 128, kSwizzle128);
@@ -230,27 +280,28 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       const uint32_t lv = desc_lo(smem_u32(smem + C::OFF_RING), C::BOXB);
       auto issue_s = [&](int k) {
         const int slot = (2 * k) % C::SLOTS;
-        const uint32_t lb = lk + uint32_t(slot * (C::TILEB >> 4));
+        const uint32_t lb = lk + uint32_t((slot * C::TILEB) >> 4);
         if (leader) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = uint32_t(((kk / 4) * C::BOXB + (kk % 4) * 32) >> 4);
             mma_ss(tmem + C::COL_S + (k & 1) * kTile, desc_make(lq + off, HI), desc_make(lb + off, HI), C::IDESC_S, kk > 0);
           }
-          mma_commit(empty + slot);
           mma_commit(s_full + (k & 1));
+          mma_commit(empty + slot);
         }
         __syncwarp();
       };
-      auto issue_pv = [&](int k) {
+      auto issue_pv = [&](int g, int k) {
         const int slot = (2 * k + 1) % C::SLOTS;
-        const uint32_t lb = lv + uint32_t(slot * (C::TILEB >> 4));
+        const uint32_t lb = lv + uint32_t((slot * C::TILEB + g * 64 * 128) >> 4);
         if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
-            mma_ts(tmem + C::COL_O + (k & 1) * D, tmem + C::COL_S + (k & 1) * kTile + kk * 8,
-                   desc_make(lb + uint32_t((kk * 16 * 128) >> 4), HI), C::IDESC_O, (k > 1 || kk > 0) ? 1u : 0u);
-          mma_commit(empty + slot);
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ts(tmem + C::COL_O + g * D, tmem + C::COL_S + (k & 1) * kTile + g * 64 + kk * 8,
+                   desc_make(lb + uint32_t((kk * 16 * 128) >> 4), HI), C::IDESC_O, (k > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(o_ready + g);
+          if (g == 1) mma_commit(empty + slot);
         }
         __syncwarp();
       };
@@ -262,13 +313,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         issue_s(k);
       }
       for (int k = 0; k < nt && ok; ++k) {
-        ok = mbar_wait(p_full + (k & 1), (k >> 1) & 1, c.status, 75);
-        if (ok) ok = mbar_wait(full + (2 * k + 1) % C::SLOTS, ((2 * k + 1) / C::SLOTS) & 1, c.status, 76);
-        if (!ok) break;
-        tc_fence_after();
-        issue_pv(k);
-        if (k + 2 < nt) {
-          // The MMAs run in the order they are issued: S takes P's place after P V has read it.
+        for (int g = 0; g < 2 && ok; ++g) {
+          ok = mbar_wait(p_full + g * 2 + (k & 1), (k >> 1) & 1, c.status, 75);
+          if (ok && g == 0) ok = mbar_wait(full + (2 * k + 1) % C::SLOTS, ((2 * k + 1) / C::SLOTS) & 1, c.status, 76);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(g, k);
+        }
+        if (ok && k + 2 < nt) {
+          // MMAs run in the order they are issued: S takes P's place after P V has read it. The softmax has S of tile
+          // k + 1 to work on meanwhile.
           ok = mbar_wait(full + (2 * k + 4) % C::SLOTS, ((2 * k + 4) / C::SLOTS) & 1, c.status, 77);
           if (!ok) break;
           tc_fence_after();
@@ -277,234 +331,304 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       }
       mma_commit_w(o_done);
       mbar_wait(o_done, 0, c.status, 78);  // every MMA has completed before TMEM is released
-    } else if (warp == 13) {
+    } else if (warp < kWarpField + 2) {
       // ----------------------------------------------------------------------- the keys' field and scales ----
+      // Per key, with b' = beta log2(e) and lv = log2 of V's scale (0 in fp16): the bias plus lv of a row is the smaller
+      // (b' < 0: the larger) of a = b' min(SUF - psi, 0) + lv and b' M + e, e = -b' psi + lv; -inf where there is no key.
+      const float bias = p.beta[h] * kLog2e;
+      // Two warps take alternate tiles; each also reads the phi of the tiles between its own, for the minimum.
+      const int first = warp - kWarpField;
       float mid = t1 * kTile < p.prefix_len ? later_min(c, p.prefix_table, h, t1 * kTile, p.prefix_len) : kInf;
-      float f[4], ps[4], ks[4], vs[4];
+      float4 f4, ps4, ks4, vs4, skip4;  // this tile's four keys of the lane; phi of the next tile's
       int64_t at = -1;
-      auto load = [&](int tile) {
-        // Four keys a lane, which lie in one page.
+      const float4 none = make_float4(kInf, kInf, kInf, kInf), zero4 = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto slot4 = [&](int pid, int tile) -> int64_t {
+        // Four keys a lane lie in one page, at a multiple of four (16 bytes in the float arrays).
         const int pos = tile * kTile + lane * 4;
-        at = pos < p.prefix_len ? slot_of(c, p.prefix_table, h, pos) : -1;
+        return tile >= t0 && pos < p.prefix_len ? slot_in(c, pid, h, pos) : -1;
+      };
+      auto page_of = [&](int tile) {
+        const int pos = tile * kTile + lane * 4;
+        return tile >= t0 && pos < p.prefix_len ? p.prefix_table[pos >> c.page_shift] : 0;
+      };
+      int tile = t1 - 1 - first;
+      if (first == 1) {  // the first warp's first tile comes after this one's
+        const int64_t s0 = slot4(page_of(t1 - 1), t1 - 1);
+        float4 x = s0 >= 0 ? *reinterpret_cast<const float4*>(c.phi + s0) : none;
+        const int left = p.prefix_len - (t1 - 1) * kTile - lane * 4;
+        if (left < 4) x.w = kInf;
+        if (left < 3) x.z = kInf;
+        if (left < 2) x.y = kInf;
+        float all;
+        suffix_min(fminf(fminf(x.x, x.y), fminf(x.z, x.w)), all);
+        mid = fminf(mid, all);
+      }
+      int pid = page_of(tile), pid_skip = page_of(tile - 1);  // a pair of tiles ahead of the values
+      auto load = [&]() {
+        at = slot4(pid, tile);
+        const int64_t next = slot4(pid_skip, tile - 1);
+        f4 = at >= 0 ? *reinterpret_cast<const float4*>(c.phi + at) : none;
+        skip4 = next >= 0 ? *reinterpret_cast<const float4*>(c.phi + next) : none;  // never the last, partial tile
+        ps4 = at >= 0 ? *reinterpret_cast<const float4*>(c.psi + at) : zero4;
+        if constexpr (kInt8) {
+          ks4 = at >= 0 ? *reinterpret_cast<const float4*>(c.ks + at) : zero4;
+          vs4 = at >= 0 ? *reinterpret_cast<const float4*>(c.vs + at) : zero4;
+        }
+        pid = page_of(tile - 2);
+        pid_skip = page_of(tile - 3);
+      };
+      load();
+      for (int k = first; k < nt; k += 2) {
+        const int st = k % kParStages;
+        if (k >= kParStages && !mbar_wait(par_empty + st, ((k / kParStages) - 1) & 1, c.status, 79)) break;
+        const int left = at < 0 ? 0 : p.prefix_len - tile * kTile - lane * 4;  // keys of this lane that exist
+        float f[4] = {f4.x, f4.y, f4.z, f4.w}, ps[4] = {ps4.x, ps4.y, ps4.z, ps4.w};
+        float ks[4], vs[4];
+        if constexpr (kInt8) {
+          ks[0] = ks4.x, ks[1] = ks4.y, ks[2] = ks4.z, ks[3] = ks4.w;
+          vs[0] = vs4.x, vs[1] = vs4.y, vs[2] = vs4.z, vs[3] = vs4.w;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool ok = at >= 0 && pos + j < p.prefix_len;
-          f[j] = ok ? c.phi[at + j] : kInf;
-          ps[j] = ok ? c.psi[at + j] : 0.f;
-          if constexpr (kInt8) {
-            ks[j] = ok ? c.ks[at + j] : 0.f;
-            vs[j] = ok ? c.vs[at + j] : 0.f;
+          if (j >= left) {
+            f[j] = kInf;
+            ps[j] = 0.f;
+            if constexpr (kInt8) ks[j] = vs[j] = 0.f;
           }
         }
-      };
-      load(t1 - 1);
-      for (int k = 0; k < nt; ++k) {
-        const int st = k % kParStages, tile = t1 - 1 - k;
-        if (k >= kParStages && !mbar_wait(par_empty + st, ((k / kParStages) - 1) & 1, c.status, 79)) break;
-        float all;
+        float all, all_skip;
         float suf = fminf(suffix_min(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), all), mid);
-        mid = fminf(mid, all);
-        float a[4], fac[4], lv[4], rv[4];
+        all_skip = fminf(fminf(skip4.x, skip4.y), fminf(skip4.z, skip4.w));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all_skip = fminf(all_skip, __shfl_xor_sync(0xffffffffu, all_skip, o));
+        mid = fminf(mid, fminf(all, all_skip));
+        float a[4], e[4], fac[4], rv[4];
 #pragma unroll
         for (int j = 3; j >= 0; --j) {
-          const bool ok = at >= 0 && tile * kTile + lane * 4 + j < p.prefix_len;
-          a[j] = ok ? fminf(suf - ps[j], 0.f) : 0.f;
-          suf = fminf(suf, f[j]);
-          lv[j] = ok ? 0.f : -kInf;
+          const bool ok = j < left;
+          float lv = 0.f;
           if constexpr (kInt8) {
             const float v = fmaxf(vs[j], 0x1p-90f);
             fac[j] = ks[j] * p.scale2;
-            if (ok) lv[j] = lg2(v);
+            lv = lg2(v);
             rv[j] = ok ? rcp_approx_f(v) : 0.f;
           }
+          a[j] = ok ? fmaf(bias, fminf(suf - ps[j], 0.f), lv) : -kInf;
+          e[j] = ok ? fmaf(-bias, ps[j], lv) : -kInf;
+          suf = fminf(suf, f[j]);
         }
         float* out = reinterpret_cast<float*>(smem + C::OFF_PAR + st * C::PARB);
 #pragma unroll
         for (int j = 0; j < 4; j += 2) {
           const int pair = lane * 2 + j / 2;
-          reinterpret_cast<float4*>(out)[pair] = make_float4(-ps[j], -ps[j + 1], a[j], a[j + 1]);
+          reinterpret_cast<float4*>(out)[pair] = make_float4(e[j], e[j + 1], a[j], a[j + 1]);
           if constexpr (kInt8) {
-            reinterpret_cast<float4*>(out + kTile * 2)[pair] = make_float4(fac[j], fac[j + 1], lv[j], lv[j + 1]);
-            reinterpret_cast<float2*>(out + kTile * 4)[pair] = make_float2(rv[j], rv[j + 1]);
-          } else {
-            reinterpret_cast<float2*>(out + kTile * 2)[pair] = make_float2(lv[j], lv[j + 1]);
+            reinterpret_cast<float2*>(out + kTile * 2)[pair] = make_float2(fac[j], fac[j + 1]);
+            reinterpret_cast<float2*>(out + kTile * 3)[pair] = make_float2(rv[j], rv[j + 1]);
           }
         }
         mbar_arrive(par_full + st);
-        if (k + 1 < nt) load(tile - 1);
+        tile -= 2;
+        if (k + 2 < nt) load();
       }
     }
   } else {
     // ------------------------------------------------------------------------------------------- softmax ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;" ::: "memory");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;" ::: "memory");
     const int g = warp >> 2;
     {
       // Q into shared memory, each copy of the rows; rows that are not there are zero.
       const __half* q = static_cast<const __half*>(p.q) + h * p.sq.h;
       const uint32_t sq = smem_u32(smem + C::OFF_Q);
-      for (int e = threadIdx.x; e < kTile * (D / 8); e += 256) {
-        const int r = e / (D / 8), ch = e % (D / 8), lr = r % RP;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (lr < rows) {
-          const int i = r0 + lr, b = i / p.n;
+      constexpr int kAhead = D / 16;  // all of this thread's
+      for (int e0 = threadIdx.x; e0 < kTile * (D / 8); e0 += kAhead * 256) {
+        uint32_t x[kAhead][4];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int e = e0 + a * 256, r = e / (D / 8), ch = e % (D / 8), lr = r % RP;
+          const int i = r0 + min(lr, rows - 1), b = i / p.n;
           const __half* row = q + b * p.sq.b + (i - b * p.n) * p.sq.t + ch * 8 * p.sq.d;
-          uint32_t x[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (p.q_pairs) {
-              x[j] = *reinterpret_cast<const uint32_t*>(row + 2 * j);
+              x[a][j] = *reinterpret_cast<const uint32_t*>(row + 2 * j);
             } else {
               const __half2 v = __halves2half2(row[2 * j * p.sq.d], row[(2 * j + 1) * p.sq.d]);
-              x[j] = *reinterpret_cast<const uint32_t*>(&v);
+              x[a][j] = *reinterpret_cast<const uint32_t*>(&v);
             }
+            if (lr >= rows) x[a][j] = 0;
           }
-          w = make_uint4(x[0], x[1], x[2], x[3]);
         }
-        st_shared16(sq + tile_chunk(r, ch), w);
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int e = e0 + a * 256;
+          st_shared16(sq + tile_chunk(e / (D / 8), e % (D / 8)), make_uint4(x[a][0], x[a][1], x[a][2], x[a][3]));
+        }
       }
       fence_async_proxy();
       mbar_arrive(q_full);
     }
     const int lrow = (warp & 3) * 32 + lane;  // TMEM lane
     const int copy = lrow / RP, lr = lrow % RP;
-    constexpr int CW = kTile / REP;           // this copy's keys of a tile
-    const int c0 = copy * CW;
+    constexpr int CW = kTile / 2 / REP;       // this copy's keys of the group's half tile
+    const int c0 = copy * CW;                 // within the half tile
     const bool busy = lr - lane < rows;       // some row of this warp exists (RP is a multiple of 32)
     const uint32_t tl = tmem + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t tS = tl + C::COL_S + g * kTile, tO = tl + C::COL_O + g * D;
+    const uint32_t tO = tl + C::COL_O + g * D;
     pdl_wait();  // row_min
     pdl_launch_dependents();
     const float low = lr < rows ? p.row_min[int64_t(h) * R + r0 + lr] : kInf;
     const float bias = p.beta[h] * kLog2e;
-    const float2 low2 = make_float2(low, low), bias2 = make_float2(bias, bias), sc2 = make_float2(p.scale2, p.scale2);
+    const float2 low2 = make_float2(bias * low, bias * low), sc2 = make_float2(p.scale2, p.scale2);
     float m = -kInf;
     float2 l2 = make_float2(0.f, 0.f);
     bool ok = true;
-    for (int k = g; k < nt && ok; k += 2) {
-      const int st = k % kParStages;
-      ok = mbar_wait(par_full + st, (k / kParStages) & 1, c.status, 80);
-      if (ok) ok = mbar_wait(s_full + g, (k >> 1) & 1, c.status, 81);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      if (busy) {
-        const float* par = reinterpret_cast<const float*>(smem + C::OFF_PAR + st * C::PARB);
-        float s[CW];
+    auto walk = [&](auto negative) {
+      auto nearer = [](float x, float y) { return decltype(negative)::value ? fmaxf(x, y) : fminf(x, y); };
+      for (int k = 0; k < nt; ++k) {
+        const int st = k % kParStages;
+        ok = mbar_wait(par_full + st, (k / kParStages) & 1, c.status, 80);
+        if (ok) ok = mbar_wait(s_full + (k & 1), (k >> 1) & 1, c.status, 81);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (busy) {
+          const uint32_t tS = tl + C::COL_S + (k & 1) * kTile + g * 64;
+          const float* par = reinterpret_cast<const float*>(smem + C::OFF_PAR + st * C::PARB);
+          const int pair0 = (g * 64 + c0) >> 1;
+          float s[CW];
+          if constexpr (CW >= 32) {
 #pragma unroll
-        for (int i = 0; i < CW; i += 32) tmem_ld32(tS + c0 + i, s + i);
-        tmem_ld_wait();
-        float m4[4] = {-kInf, -kInf, -kInf, -kInf};
-#pragma unroll
-        for (int i = 0; i < CW; i += 2) {
-          const int pair = (c0 + i) >> 1;
-          const float4 x = reinterpret_cast<const float4*>(par)[pair];
-          const float2 t = __fadd2_rn(low2, make_float2(x.x, x.y));
-          const float2 b = make_float2(fminf(x.z, t.x), fminf(x.w, t.y));
-          float2 z;
-          if constexpr (kInt8) {
-            const float4 y = reinterpret_cast<const float4*>(par + kTile * 2)[pair];
-            z = __ffma2_rn(make_float2(s[i], s[i + 1]), make_float2(y.x, y.y), __ffma2_rn(bias2, b, make_float2(y.z, y.w)));
+            for (int i = 0; i < CW; i += 32) tmem_ld32(tS + c0 + i, s + i);
           } else {
-            const float2 lv = reinterpret_cast<const float2*>(par + kTile * 2)[pair];
-            z = __ffma2_rn(make_float2(s[i], s[i + 1]), sc2, __ffma2_rn(bias2, b, lv));
+            tmem_ld16(tS + c0, s);
           }
-          s[i] = z.x;
-          s[i + 1] = z.y;
-          m4[(i >> 1) & 3] = fmax3f(m4[(i >> 1) & 3], z.x, z.y);
-        }
-        const float mt = fmaxf(fmax3f(m4[0], m4[1], m4[2]), m4[3]);
-        // A new maximum only when it grows by more than 8 (log2 units); O holds the sums up to this group's last tile.
-        const bool grow = mt > m + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float mn = grow ? mt : m, alpha = grow ? state_weight(m, mn) : 1.f;
-          m = mn;
-          l2.x *= alpha;
-          l2.y *= alpha;
-          if (k > 1) {
+          tmem_ld_wait();
+          float m4[4] = {-kInf, -kInf, -kInf, -kInf};
 #pragma unroll
-            for (int cc = 0; cc < D; cc += 16) {
-              float o[16];
-              tmem_ld16(tO + cc, o);
-              tmem_ld_wait();
+          for (int i = 0; i < CW; i += 2) {
+            const int pair = pair0 + (i >> 1);
+            const float4 x = reinterpret_cast<const float4*>(par)[pair];
+            const float2 t = __fadd2_rn(low2, make_float2(x.x, x.y));
+            const float2 b = make_float2(nearer(x.z, t.x), nearer(x.w, t.y));
+            const float2 f2 = kInt8 ? reinterpret_cast<const float2*>(par + kTile * 2)[pair] : sc2;
+            const float2 z = __ffma2_rn(make_float2(s[i], s[i + 1]), f2, b);
+            s[i] = z.x;
+            s[i + 1] = z.y;
+            m4[(i >> 1) & 3] = fmax3f(m4[(i >> 1) & 3], z.x, z.y);
+          }
+          const float mt = fmaxf(fmax3f(m4[0], m4[1], m4[2]), m4[3]);
+          // A new maximum only when it grows by more than 8 (log2 units).
+          const bool grow = mt > m + 8.f;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float mn = grow ? mt : m, alpha = grow ? state_weight(m, mn) : 1.f;
+            m = mn;
+            l2.x *= alpha;
+            l2.y *= alpha;
+            if (k > 0) {
+              ok = mbar_wait(o_ready + g, (k - 1) & 1, c.status, 84);  // O holds the tiles before this one
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= alpha;
-              tmem_st16(tO + cc, reinterpret_cast<const uint32_t*>(o));
+              for (int cc = 0; cc < D; cc += 16) {
+                float o[16];
+                tmem_ld16(tO + cc, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                tmem_st16(tO + cc, reinterpret_cast<const uint32_t*>(o));
+              }
             }
           }
-        }
-        const float ref = m == -kInf ? 0.f : -m;
-        const float2 ref2 = make_float2(ref, ref);
+          const float ref = m == -kInf ? 0.f : -m;
+          const float2 ref2 = make_float2(ref, ref);
+          uint32_t pk[CW / 2];
 #pragma unroll
-        for (int cc = 0; cc < CW; cc += 32) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 x = __fadd2_rn(make_float2(s[cc + e], s[cc + e + 1]), ref2);
+          for (int e = 0; e < CW; e += 2) {
+            const float2 x = __fadd2_rn(make_float2(s[e], s[e + 1]), ref2);
             const float2 pp = make_float2(ex2(x.x), ex2(x.y));
             if constexpr (kInt8)
-              l2 = __ffma2_rn(pp, reinterpret_cast<const float2*>(par + kTile * 4)[(c0 + cc + e) >> 1], l2);
+              l2 = __ffma2_rn(pp, reinterpret_cast<const float2*>(par + kTile * 3)[pair0 + (e >> 1)], l2);
             else
               l2 = __fadd2_rn(l2, pp);
             pk[e / 2] = pack2(pp.x, pp.y);
           }
-          tmem_st16(tS + (c0 + cc) / 2, pk);
-        }
-        if constexpr (REP > 1) {
-          // The other copies' keys count nothing here.
-          const uint32_t zero[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+          if constexpr (CW == 64) {
+            tmem_st32(tS, pk);
+          } else {
+            // The keys of the other copies count nothing here.
+            const uint32_t zero[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-          for (int cc = 0; cc < kTile; cc += 32)
-            if (cc / CW != copy) tmem_st16(tS + cc / 2, zero);
+            for (int j = 0; j < REP; ++j) {
+              if constexpr (CW == 32) {
+                if (j != copy) tmem_st16(tS + j * 16, zero);
+              } else {
+                if (j != copy) tmem_st8(tS + j * 8, zero);
+              }
+            }
+            if constexpr (CW == 32)
+              tmem_st16(tS + c0 / 2, pk);
+            else
+              tmem_st8(tS + c0 / 2, pk);
+          }
+          tmem_st_wait();
         }
-        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(par_empty + st);
+        mbar_arrive(p_full + g * 2 + (k & 1));
       }
-      tc_fence_before();
-      mbar_arrive(par_empty + st);
-      mbar_arrive(p_full + g);
-    }
+    };
+    if (bias < 0.f)
+      walk(std::true_type{});
+    else
+      walk(std::false_type{});
     // The states of both groups and all copies, in the ring's place once every MMA has completed.
-    if (ok) ok = mbar_wait(o_done, 0, c.status, 82);
-    ok = __all_sync(0xffffffffu, ok);
+    mbar_wait(o_done, 0, c.status, 82);
     tc_fence_after();
-    float* sO = reinterpret_cast<float*>(smem + C::OFF_RING);
+    float* sO = reinterpret_cast<float*>(smem + C::OFF_RING);  // [state][D + 4]
     float* ml = reinterpret_cast<float*>(smem + C::OFF_ML);
-    const int state = (g * REP + copy) * RP + lr;  // = g 128 + lrow
-    const bool any = ok && g < nt;                 // this group has had a tile
-    ml[state] = any ? m : -kInf;
-    ml[256 + state] = any ? l2.x + l2.y : 0.f;
-#pragma unroll 1
-    for (int cc = 0; cc < D; cc += 32) {
-      float o[32];
-      if (any) {
+    const int state = g * kTile + lrow;  // = (g REP + copy) RP + lr
+    ml[state] = m;
+    ml[256 + state] = l2.x + l2.y;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    float M = -kInf, l = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2 * REP; ++s) M = fmaxf(M, ml[s * RP + lr]);
+#pragma unroll
+    for (int s = 0; s < 2 * REP; ++s) l += state_weight(ml[s * RP + lr], M) * ml[256 + s * RP + lr];
+    const float w = state_weight(m, M);
+    if (busy) {
+#pragma unroll
+      for (int cc = 0; cc < D; cc += 32) {
+        float o[32];
         tmem_ld32(tO + cc, o);
         tmem_ld_wait();
-      }
 #pragma unroll
-      for (int e = 0; e < 32; ++e) sO[state * (D + 1) + cc + e] = any ? o[e] : 0.f;
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<float4*>(sO + state * (D + 4) + cc + e) =
+              make_float4(o[e] * w, o[e + 1] * w, o[e + 2] * w, o[e + 3] * w);
+      }
     }
     tc_fence_before();
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    for (int e = threadIdx.x; e < rows * D; e += 256) {
-      const int r = e / D, d = e - r * D;
-      float M = -kInf, l = 0.f, o = 0.f;
-#pragma unroll
-      for (int s = 0; s < 2 * REP; ++s) M = fmaxf(M, ml[s * RP + r]);
+    const int64_t out = (int64_t(h) * R + r0) * p.chunks + blockIdx.x;  // of row 0; rows are p.chunks apart
+    if (g == 0 && copy == 0 && lr < rows)
+      *reinterpret_cast<float2*>(p.part_ml + (out + int64_t(lr) * p.chunks) * 2) = make_float2(M, l);
+#pragma unroll 2
+    for (int e = threadIdx.x; e < rows * (D / 4); e += 256) {
+      const int r = e / (D / 4), d = e % (D / 4) * 4;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int s = 0; s < 2 * REP; ++s) {
-        const float w = state_weight(ml[s * RP + r], M);
-        l += w * ml[256 + s * RP + r];
-        o += w * sO[(s * RP + r) * (D + 1) + d];
+        const float4 x = *reinterpret_cast<const float4*>(sO + (s * RP + r) * (D + 4) + d);
+        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
       }
-      const int64_t at = (int64_t(h) * R + r0 + r) * p.chunks + blockIdx.x;
-      p.part_o[at * D + d] = o;
-      if (d == 0) {
-        p.part_ml[at * 2] = M;
-        p.part_ml[at * 2 + 1] = l;
-      }
+      *reinterpret_cast<float4*>(p.part_o + (out + int64_t(r) * p.chunks) * D + d) = o;
     }
   }
   __syncthreads();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == kWarpMma) tmem_dealloc(tmem, 512);
 }
 
 template <int D, bool kInt8>

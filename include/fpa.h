@@ -134,8 +134,8 @@ typedef struct FpaCache {
   int32_t n_pages, H;
   int32_t page_size;        /* 32, 64, 128 or 256 */
   int32_t D;                /* 16, 32, 64, 128 or 256 */
-  void* k;                  /* [n_pages, H, page_size, D], 16-byte aligned */
-  void* v;                  /* [n_pages, H, page_size, D], 16-byte aligned */
+  void* k;                  /* [n_pages, H, page_size, D]; k, v, the scales, phi and psi are 16-byte aligned */
+  void* v;                  /* [n_pages, H, page_size, D] */
   float* k_scale;           /* [n_pages, H, page_size] (int8 storage; else ignored) */
   float* v_scale;
   float* phi;               /* [n_pages, H, page_size] */
