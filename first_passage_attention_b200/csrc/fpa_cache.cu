@@ -1,20 +1,54 @@
 // The paged cache: tokens quantised as they are written, and read back.
 //
-// Both are one pass over the data and bound by its bytes. Eight elements of a row belong to one lane (16 bytes of
-// fp16), D / 8 lanes to a row. int8: the row's largest magnitude `top` by shuffles, scale = top / 127, code =
-// rint((127 x) / top): for fp16 inputs 127 x is exact in float32 and the quotient of two 18- and 11-bit integers never
-// comes closer to a half without being one than float32 resolves, so every code is the correctly rounded one. The
-// quotient is taken as a product with 1 / top, which is off by less than 2^-14 for |quotient| <= 127, and as a division
-// only where the product lies that close to a half. Stored is code + 128. Each thread has the loads of several rows in
-// flight before it works on the first.
-// A block of the append owns one page of one (sequence, head): it alone writes the page's minimum of phi.
+// Both are one pass over the data and bound by its bytes, short calls by a chain of look-ups. Eight elements of a row
+// belong to one lane (16 bytes of fp16), D / 8 lanes to a row; a thread has the loads of several rows in flight. int8: the
+// row's largest magnitude `top` by shuffles, scale = top / 127, code = rint((127 x) / top): for fp16 inputs 127 x is
+// exact in float32 and the quotient of two 18- and 11-bit integers never comes closer to a half without being one than
+// float32 resolves, so every code is the correctly rounded one. The quotient is taken as a product with 127 / top, which
+// is off by less than 2^-14 for |quotient| <= 127, and as a division only where the product lies that close to a half.
+// Rounding and conversion go through sums with 1.5 2^23 (codes sit in the sum's low bits): conversion instructions run
+// at a quarter of the rate. Stored is code + 128. A block of the append owns one page of one (sequence, head): it alone
+// writes the page's minimum of phi.
 #include "fpa_serve.h"
 
 namespace fpa {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kReadThreads = 128;
+constexpr int kMaxThreads = 256;
 constexpr int kAhead = 4;  // rows whose loads a thread has in flight
+
+// Codes + 128 of eight elements from their row's largest magnitude, four to a word.
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], float top) {
+  constexpr float kRound = 12582912.f + 128.f;  // 1.5 2^23: a sum with it is rounded to an integer, even on ties
+  const float k = 127.f * rcp_approx_f(top);
+  uint32_t w[8];
+  float off = 0.f;  // largest distance from an integer
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float c = __fmul_rn(x[j], k), r = __fadd_rn(c, kRound);
+    off = fmaxf(off, fabsf(__fsub_rn(c, __fsub_rn(r, kRound))));
+    w[j] = __float_as_uint(r);
+  }
+  if (!(off < 0.5f - 0x1p-14f) || !(top < 0x1p100f)) {  // near a half, or the reciprocal leaves float32's normal range
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      w[j] = min(max(__float2int_rn(__fdiv_rn(__fmul_rn(x[j], 127.f), top)), -127), 127) + 128;
+  }
+  auto four = [&](int j) {
+    return __byte_perm(__byte_perm(w[j], w[j + 1], 0x0040), __byte_perm(w[j + 2], w[j + 3], 0x0040), 0x5410);
+  };
+  return make_uint2(four(0), four(4));
+}
+
+// Values of four codes.
+__device__ __forceinline__ void decode4(uint32_t w, float scale, float* x) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float u = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7650u | j));  // 2^23 + code + 128
+    x[j] = __fmul_rn(__fsub_rn(u, 8388608.f + 128.f), scale);
+  }
+}
 
 // Eight consecutive elements of a row in float32.
 template <typename T>
@@ -74,11 +108,11 @@ struct AppendParams {
 
 // T: type of k and v; kInt8: codes and scales, else rows as they are.
 template <typename T, bool kInt8>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 4) append_kernel(const __grid_constant__ AppendParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const CacheView& c = p.c;
-  const int h = blockIdx.y, b = blockIdx.z, page = 1 << c.page_shift;
+  const int h = blockIdx.y, b = blockIdx.z, page = 1 << c.page_shift, threads = blockDim.x;
   const int start = p.start[b];
   const int count = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
   if (count == 0) return;
@@ -93,89 +127,101 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   const int i0 = int(max(first - start, int64_t(0))), i1 = int(min(first + page - start, int64_t(count)));
   if (i0 >= i1) return;
   const int pid = pg < p.max_pages ? p.table[b * p.table_stride + pg] : -1;
+  const int slot0 = int(start + i0 - first), tokens = i1 - i0;
+  // Half of the block takes K, half V: thread (sub, e0) the eight elements from e0 on of tokens sub, sub + rows, ...
+  const int lanes = c.D >> 3, rows = threads / 2 / lanes;
+  const int which = int(threadIdx.x) >= threads / 2 ? 1 : 0, tid = threadIdx.x - which * (threads / 2);
+  const int sub = tid / lanes, e0 = (tid - sub * lanes) * 8;
+  const Str4 st = p.st[which];
+  const T* src = static_cast<const T*>(p.src[which]) + b * st.b + h * st.h + (i0 + sub) * st.t + e0 * st.d;
+  const int64_t step = rows * st.t;
+  const bool vec = p.vec[which] != 0;
+  float x[kAhead][8];
+  auto load_rows = [&](int t0) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[a][j] = 0.f;
+      if (t0 + a * rows + sub < tokens) load8(src + a * step, st.d, vec, x[a]);
+    }
+    src += kAhead * step;
+  };
+  // What does not depend on the page's id travels with it.
+  load_rows(0);
+  const float* src_phi = p.phi + b * p.sphi.b + h * p.sphi.h;
+  const float* src_psi = p.psi + b * p.spsi.b + h * p.spsi.h;
+  const bool mine = int(threadIdx.x) < tokens;
+  const float phi0 = mine ? src_phi[(i0 + int(threadIdx.x)) * p.sphi.t] : kInf;
+  const float psi0 = mine ? src_psi[(i0 + int(threadIdx.x)) * p.spsi.t] : 0.f;
   if (unsigned(pid) >= unsigned(c.n_pages)) {
     if (threadIdx.x == 0) report_bad_page(c.status, kSiteAppend);
     return;
   }
   const int64_t base = (int64_t(pid) * c.H + h) << c.page_shift;  // pool index of the page's slot 0
-  const int slot0 = int(start + i0 - first);
-  const int lanes = c.D >> 3, rows = kThreads / lanes;
-  const int sub = threadIdx.x / lanes, e0 = (threadIdx.x - sub * lanes) * 8;
-  const int tokens = i1 - i0;
-  // Rows 0 .. tokens - 1 are K's, the rest V's. Whole warps stay in the loop for the shuffles.
-  for (int r0 = 0; r0 < 2 * tokens; r0 += kAhead * rows) {
-    float x[kAhead][8];
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int r = r0 + a * rows + sub;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[a][j] = 0.f;
-      if (r < 2 * tokens) {
-        const int which = r >= tokens ? 1 : 0;
-        const Str4& st = p.st[which];
-        load8(static_cast<const T*>(p.src[which]) + b * st.b + h * st.h + (i0 + r - which * tokens) * st.t + e0 * st.d,
-              st.d, p.vec[which] != 0, x[a]);
-      }
-    }
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      if (r0 + a * rows >= 2 * tokens) break;
-      const int r = r0 + a * rows + sub;
-      const bool ok = r < 2 * tokens;
-      const int which = ok && r >= tokens ? 1 : 0;
-      const int64_t at = base + slot0 + r - which * tokens;
-      if constexpr (kInt8) {
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[a][j]));
-        for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // Scales stay at or above 2^-90, so that their inverses sum up in float32 (see fpa_decode_mma.cu); a row of
-        // zeros takes that smallest scale, so that it does not outweigh small rows there.
-        top = fmaxf(top, 127.f * 0x1p-90f);
-        const float inv = __frcp_rn(top);
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float y = __fmul_rn(x[a][j], 127.f);
-          float c_ = __fmul_rn(y, inv);
-          int code = __float2int_rn(c_);
-          // Near a half, or with a reciprocal or product out of float32's normal range: the division itself.
-          if (!(fabsf(fabsf(c_ - float(code)) - 0.5f) > 0x1p-13f) || !(top < 0x1p100f))
-            code = min(max(__float2int_rn(__fdiv_rn(y, top)), -127), 127);
-          w[j >> 2] |= uint32_t(code + 128) << (8 * (j & 3));
-        }
-        if (ok) {
-          char* dst = const_cast<char*>(static_cast<const char*>(which ? c.v : c.k)) + at * c.D + e0;
-          *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-          if (e0 == 0) const_cast<float*>(which ? c.vs : c.ks)[at] = __fdiv_rn(top, 127.f);
-        }
-      } else if (ok) {
-        store8(const_cast<T*>(static_cast<const T*>(which ? c.v : c.k)) + at * c.D + e0, x[a]);
-      }
-    }
-  }
   // The field, and the page's minimum over the slots up to the last one written.
-  float low = kInf;
   float* phi = const_cast<float*>(c.phi) + base;
-  for (int s = threadIdx.x; s < slot0 + tokens; s += kThreads) {
-    float f;
-    if (s < slot0) {
-      f = phi[s];
-    } else {
-      const int i = i0 + s - slot0;
-      f = p.phi[b * p.sphi.b + h * p.sphi.h + i * p.sphi.t];
-      phi[s] = f;
-      const_cast<float*>(c.psi)[base + s] = p.psi[b * p.spsi.b + h * p.spsi.h + i * p.spsi.t];
-    }
+  float* psi = const_cast<float*>(c.psi) + base + slot0;
+  float low = phi0;
+  if (mine) {
+    phi[slot0 + threadIdx.x] = phi0;
+    psi[threadIdx.x] = psi0;
+  }
+  for (int i = threadIdx.x + threads; i < tokens; i += threads) {
+    const float f = src_phi[(i0 + i) * p.sphi.t];
+    phi[slot0 + i] = f;
+    psi[i] = src_psi[(i0 + i) * p.spsi.t];
     low = fminf(low, f);
   }
-  __shared__ float warp_low[kThreads / 32];
+  for (int s = threadIdx.x; s < slot0; s += threads) low = fminf(low, phi[s]);
+  // Whole warps stay in the loop for the shuffles.
+  char* dst = const_cast<char*>(static_cast<const char*>(which ? c.v : c.k)) +
+              ((base + slot0 + sub) * c.D + e0) * int(kInt8 ? 1 : sizeof(T));
+  float* scales = const_cast<float*>(which ? c.vs : c.ks) + base + slot0 + sub;
+  const int dst_step = rows * c.D * int(kInt8 ? 1 : sizeof(T));
+  for (int t0 = 0; t0 < tokens; t0 += kAhead * rows) {
+    if (t0 > 0) load_rows(t0);
+    float top[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      if (t0 + a * rows >= tokens) break;
+      const bool ok = t0 + a * rows + sub < tokens;
+      if constexpr (kInt8) {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[a][j]));
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+          if (o < lanes) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        // Scales stay at or above 2^-90, so that their inverses sum up in float32 (see fpa_decode_mma.cu); a row of
+        // zeros takes that smallest scale, so that it does not outweigh small rows there.
+        top[a] = fmaxf(m, 127.f * 0x1p-90f);
+        const uint2 w = encode8(x[a], top[a]);
+        if (ok) *reinterpret_cast<uint2*>(dst + a * dst_step) = w;
+      } else if (ok) {
+        store8(reinterpret_cast<T*>(dst + a * dst_step), x[a]);
+      }
+    }
+    if constexpr (kInt8) {
+      // Lane j of a row's lanes divides for the j-th row (and the rows `lanes` after it).
+      for (int a0 = 0; a0 < kAhead; a0 += lanes) {
+        const int a = a0 + (e0 >> 3);
+        float t = top[0];
+#pragma unroll
+        for (int j = 1; j < kAhead; ++j)
+          if (a == j) t = top[j];
+        if (a < kAhead && t0 + a * rows + sub < tokens) scales[a * rows] = __fdiv_rn(t, 127.f);
+      }
+    }
+    dst += kAhead * dst_step;
+    scales += kAhead * rows;
+  }
+  __shared__ float warp_low[kMaxThreads / 32];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
   if ((threadIdx.x & 31) == 0) warp_low[threadIdx.x >> 5] = low;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) low = fminf(low, warp_low[w]);
+    for (int w = 1; w < threads / 32; ++w) low = fminf(low, warp_low[w]);
     const_cast<float*>(c.pmin)[int64_t(pid) * c.H + h] = low;
   }
 }
@@ -197,7 +243,7 @@ struct ReadParams {
 constexpr int kReadRows = 64;
 
 template <typename T, bool kInt8>
-__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadParams p) {
+__global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constant__ ReadParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const CacheView& c = p.c;
@@ -220,51 +266,53 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
     }
     return ((int64_t(pid) * c.H + h) << c.page_shift) + (s & (page - 1));
   };
-  const int lanes = c.D >> 3, rows = kThreads / lanes;
+  const int lanes = c.D >> 3, rows = kReadThreads / lanes;
   const int sub = threadIdx.x / lanes, e0 = (threadIdx.x - sub * lanes) * 8;
   for (int first = i0 + sub; first < i1; first += kAhead * rows) {
     int64_t at[kAhead];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) at[a] = first + a * rows < i1 ? slot(first + a * rows) : -1;
+    const int64_t to = (out0 + first) * c.D + e0;
+    if constexpr (kInt8) {
+      uint2 w[2][kAhead];
+      float scale[2][kAhead];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const void* src = which ? c.v : c.k;
-      T* dst = static_cast<T*>(which ? p.v : p.k) + (out0 + first) * c.D + e0;
-      if constexpr (kInt8) {
-        uint2 w[kAhead];
-        float scale[kAhead];
+      for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-          w[a] = make_uint2(0, 0);
-          scale[a] = 0.f;
+          w[which][a] = make_uint2(0x80808080u, 0x80808080u);  // code 0
+          scale[which][a] = 0.f;
           if (at[a] >= 0) {
-            w[a] = __ldcs(reinterpret_cast<const uint2*>(static_cast<const char*>(src) + at[a] * c.D + e0));
-            scale[a] = (which ? c.vs : c.ks)[at[a]];
+            w[which][a] = __ldcs(reinterpret_cast<const uint2*>(static_cast<const char*>(which ? c.v : c.k) + at[a] * c.D + e0));
+            scale[which][a] = (which ? c.vs : c.ks)[at[a]];
           }
         }
 #pragma unroll
+      for (int which = 0; which < 2; ++which)
+#pragma unroll
         for (int a = 0; a < kAhead; ++a) {
           float x[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            x[j] = at[a] >= 0 ? float(int(((j < 4 ? w[a].x : w[a].y) >> (8 * (j & 3))) & 0xff) - 128) * scale[a] : 0.f;
-          if (first + a * rows < i1) store8(dst + int64_t(a) * rows * c.D, x);
+          decode4(w[which][a].x, scale[which][a], x);
+          decode4(w[which][a].y, scale[which][a], x + 4);
+          if (first + a * rows < i1) store8(static_cast<T*>(which ? p.v : p.k) + to + int64_t(a) * rows * c.D, x);
         }
-      } else {
+    } else {
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
         float x[kAhead][8];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[a][j] = 0.f;
-          if (at[a] >= 0) load8(static_cast<const T*>(src) + at[a] * c.D + e0, 1, true, x[a]);
+          if (at[a] >= 0) load8(static_cast<const T*>(which ? c.v : c.k) + at[a] * c.D + e0, 1, true, x[a]);
         }
 #pragma unroll
         for (int a = 0; a < kAhead; ++a)
-          if (first + a * rows < i1) store8(dst + int64_t(a) * rows * c.D, x[a]);
+          if (first + a * rows < i1) store8(static_cast<T*>(which ? p.v : p.k) + to + int64_t(a) * rows * c.D, x[a]);
       }
     }
   }
-  for (int i = i0 + threadIdx.x; i < i1; i += kThreads) {
+  for (int i = i0 + threadIdx.x; i < i1; i += kReadThreads) {
     const int64_t at = slot(i);
     p.phi[out0 + i] = at >= 0 ? c.phi[at] : 0.f;
     p.psi[out0 + i] = at >= 0 ? c.psi[at] : 0.f;
@@ -354,7 +402,8 @@ extern "C" FPA_API int fpa_cache_append(const FpaAppendArgs* a, void* stream) {
   const bool i8 = c.storage == FPA_STORE_I8;
   auto kernel = c.dtype == FPA_DTYPE_F16 ? (i8 ? append_kernel<__half, true> : append_kernel<__half, false>)
                                          : (i8 ? append_kernel<float, true> : append_kernel<float, false>);
-  return cuda_result(launch_pdl(kernel, grid, dim3(kThreads), 0, static_cast<cudaStream_t>(stream), p), "fpa_cache_append");
+  return cuda_result(launch_pdl(kernel, grid, dim3(a->n > 16 ? kMaxThreads : 128), 0, static_cast<cudaStream_t>(stream), p),
+                     "fpa_cache_append");
 }
 
 extern "C" FPA_API int fpa_cache_read(const FpaReadArgs* a, void* stream) {
@@ -372,5 +421,5 @@ extern "C" FPA_API int fpa_cache_read(const FpaReadArgs* a, void* stream) {
   const bool i8 = c.storage == FPA_STORE_I8;
   auto kernel = c.dtype == FPA_DTYPE_F16 ? (i8 ? read_kernel<__half, true> : read_kernel<__half, false>)
                                          : (i8 ? read_kernel<float, true> : read_kernel<float, false>);
-  return cuda_result(launch_pdl(kernel, grid, dim3(kThreads), 0, static_cast<cudaStream_t>(stream), p), "fpa_cache_read");
+  return cuda_result(launch_pdl(kernel, grid, dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream), p), "fpa_cache_read");
 }

@@ -41,9 +41,10 @@ def _int32_on(name, x, index, shape):
 def _table_on(x, index, B):
     if x.dtype != torch.int32 or x.get_device() != index:
         raise ValueError(f"block_table must be an int32 tensor on cuda:{index}")
-    if x.dim() != 2 or x.shape[0] != B or x.shape[1] < 1 or (x.stride(1) != 1 and x.shape[1] > 1):
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 2 or shape[0] != B or shape[1] < 1 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError("block_table must have shape (B, pages) with contiguous rows")
-    return x.data_ptr(), x.stride(0), x.shape[1]
+    return x.data_ptr(), stride[0], shape[1]
 
 
 def _call(fn, args, index):
@@ -113,12 +114,13 @@ class FPACache:
         there on is gone (that is also how refused drafts are taken back)."""
         lib = _lib.load()
         H, D = self.n_heads, self.head_dim
-        if k.dim() != 4 or v.shape != k.shape or k.shape[1] != H or k.shape[3] != D:
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape or shape[1] != H or shape[3] != D:
             raise ValueError(f"k and v must have shape (B, {H}, n, {D})")
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise ValueError(f"k and v must be {self.dtype}")
-        B, _, n, _ = k.shape
-        if phi.shape != k.shape[:3] or psi.shape != phi.shape:
+        B, _, n, _ = shape
+        if phi.shape != (B, H, n) or psi.shape != (B, H, n):
             raise ValueError(f"phi and psi must have shape (B, {H}, n)")
         if phi.dtype != torch.float32 or psi.dtype != torch.float32:
             raise ValueError("phi and psi must be float32")
@@ -175,9 +177,10 @@ def first_passage_decode(q, cache, block_table, lengths, beta, prefix_table=None
     batch. Equal to the last n rows of ``first_passage_attention`` over the whole sequence."""
     lib = _lib.load()
     H, D, dev = cache.n_heads, cache.head_dim, cache._index
-    if q.dim() != 4 or q.shape[1] != H or q.shape[3] != D:
+    shape = q.shape
+    if len(shape) != 4 or shape[1] != H or shape[3] != D:
         raise ValueError(f"q must have shape (B, {H}, n, {D})")
-    B, _, n, _ = q.shape
+    B, _, n, _ = shape
     if not 1 <= n <= MAX_NEW_TOKENS:
         raise ValueError(f"between 1 and {MAX_NEW_TOKENS} new tokens per call")
     if q.dtype != cache.dtype or q.get_device() != dev:
