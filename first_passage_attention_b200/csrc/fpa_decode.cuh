@@ -4,7 +4,8 @@
 //     z_ts = q_t k_s / sqrt(D) + beta min(0, min_{s<u<=t} phi_u - psi_s),   z_tt without the bias.
 // With Lb = L - n, the range minimum of a history key s < Lb splits into SUF_s = min_{s<u<Lb} phi_u, which all rows
 // share, and M_r = min_{Lb<=u<=t} phi_u, so the bias is beta min(a_s, M_r - psi_s) with a_s = min(0, SUF_s - psi_s);
-// the pairs among the n newest tokens get their minimum one by one. A prefix shared by the batch is the same thing once
+// the pairs among the n newest tokens get their minimum one by one (with n = 1 the row's own key joins the history as
+// its last: the empty range leaves it no bias). A prefix shared by the batch is the same thing once
 // more: its keys' SUF ends at the prefix's end and M_r is the minimum over the row's own tokens.
 //
 // What bounds it: the bytes of the cache, and for short histories a chain of look-ups (length, table, values) of about
@@ -230,6 +231,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
     job.end = max(L - p.n, 0);
     job.n_new = L - job.end;
     job.lead = p.n - job.n_new;
+    if (p.n == 1) {
+      // One row: its own key is the last of the history, whose empty range leaves no bias.
+      job.end = L;
+      job.n_new = 0;
+    }
   }
   job.rows = min(NQ, R - job.r0);
   job.bias = p.beta[job.h] * kLog2e;
@@ -238,7 +244,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
     const int each = tiles / units, more = tiles - each * units;
     job.t0 = u * each + min(u, more);
     job.t1 = job.t0 + each + (u < more ? 1 : 0);
-    job.last = !kPrefix && u == units - 1;
+    job.last = job.n_new > 0 && u == units - 1;
   }
   Core core(p, job, scratch, reinterpret_cast<char*>(smem));
   core.template run<kPrefix>(p, job);

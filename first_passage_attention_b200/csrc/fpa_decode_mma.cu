@@ -22,6 +22,7 @@
 #include <cuda_fp16.h>
 
 #include "fpa_decode.cuh"
+#include "fpa_sm100.cuh"
 
 namespace fpa {
 namespace {
@@ -97,14 +98,14 @@ struct MmaCore {
   // tokens, 5 rows: 64 us against 69); at D = 256 in fp16 few warps fit either way (48 us with three, 60 with two).
   static constexpr int kStages = RB < 512 ? 2 : 3;
   static constexpr int kRingBytes = kStages * kStage;   // of a warp
-  static constexpr int kCtaFloats = 0, kWarpFloats = kKeys * 5;
+  static constexpr int kCtaFloats = 0, kWarpFloats = kKeys * 4;
   static constexpr int kMinBlocks = D * NT <= 64 ? (RB <= 64 ? 5 : 4) : D * NT <= 128 ? 3 : 2;
   using Out = __half;
 
   uint32_t qf[NT][KS][2];
   float o[MT][NT][4], m[NT][2], l[NT][2], low[NT][2], zero[NT][2];
-  float4* par;    // per key of the block: a, psi, factor of the product, log2 of V's scale (-inf: no such key)
-  float* rvs;     // 1 / V's scale
+  float4* par;    // per key of the block: see field_of
+  float sign;     // of beta (1 for 0)
   uint32_t ring;  // this warp's stages
   int lane, g, t;
 
@@ -114,7 +115,6 @@ struct MmaCore {
     g = lane >> 2;
     t = lane & 3;
     par = reinterpret_cast<float4*>(scratch + warp * kWarpFloats);
-    rvs = scratch + warp * kWarpFloats + kKeys * 4;
     ring = static_cast<uint32_t>(__cvta_generic_to_shared(rings)) + warp * kRingBytes;
   }
 
@@ -296,29 +296,34 @@ struct MmaCore {
     }
   }
 
-  // Softmax of a block's scores (z + lv in log2 units) and their products with V.
-  __device__ __forceinline__ void accumulate(uint32_t st, float (&z)[SUB][NT][4], const float (&rv)[SUB][2]) {
-    bool grow = false;
+  // Softmax of a block's scores (z + lv in log2 units, less ref) and their products with V.
+  __device__ __forceinline__ void accumulate(uint32_t st, float2 (&z)[SUB][NT][2], const float (&rv)[SUB][2]) {
     float top[NT][2];
+    bool grow = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      top[nt][0] = top[nt][1] = -kInf;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        float x = -kInf;
-#pragma unroll
-        for (int b = 0; b < SUB; ++b) x = fmaxf(x, fmaxf(z[b][nt][q], z[b][nt][q + 2]));
-        top[nt][q] = x;
-        grow |= x > m[nt][q] + 8.f;
+      for (int b = 0; b < SUB; ++b) {
+        top[nt][0] = sm100::fmax3f(top[nt][0], z[b][nt][0].x, z[b][nt][1].x);
+        top[nt][1] = sm100::fmax3f(top[nt][1], z[b][nt][0].y, z[b][nt][1].y);
       }
+      // A row that has seen nothing yet (m = -inf, ref = 0) takes any maximum.
+#pragma unroll
+      for (int q = 0; q < 2; ++q) grow |= top[nt][q] > (m[nt][q] == -kInf ? -kInf : 8.f);
+    }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float shift[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          float x = fmaxf(top[nt][q], m[nt][q]);
+          const float ref = m[nt][q] == -kInf ? 0.f : m[nt][q];
+          float x = fmaxf(top[nt][q] + ref, m[nt][q]);
 #pragma unroll
           for (int o_ = 4; o_ < 32; o_ <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o_));
           const float f = state_weight(m[nt][q], x);
+          shift[q] = ref - (x == -kInf ? 0.f : x);
           m[nt][q] = x;
           l[nt][q] *= f;
 #pragma unroll
@@ -327,33 +332,34 @@ struct MmaCore {
             o[j][nt][q + 2] *= f;
           }
         }
+#pragma unroll
+        for (int b = 0; b < SUB; ++b)
+#pragma unroll
+          for (int key = 0; key < 2; ++key) z[b][nt][key] = __fadd2_rn(z[b][nt][key], make_float2(shift[0], shift[1]));
+      }
     }
     uint32_t pb[SUB][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float ref[2];
+      float2 sum = make_float2(l[nt][0], l[nt][1]);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) ref[q] = m[nt][q] == -kInf ? 0.f : m[nt][q];  // a row that has seen nothing yet
+      for (int b = 0; b < SUB; ++b)
 #pragma unroll
-      for (int b = 0; b < SUB; ++b) {
-        float e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[i] = ex2(z[b][nt][i] - ref[i & 1]);
-          if constexpr (kInt8)
-            l[nt][i & 1] = fmaf(e[i], rv[b][i >> 1], l[nt][i & 1]);
-          else
-            l[nt][i & 1] += e[i];
+        for (int key = 0; key < 2; ++key) {
+          const float2 e = make_float2(ex2(z[b][nt][key].x), ex2(z[b][nt][key].y));
+          sum = kInt8 ? __ffma2_rn(e, make_float2(rv[b][key], rv[b][key]), sum) : __fadd2_rn(sum, e);
+          pb[b][nt][key] = transpose8x8(pack_half2(e.x, e.y));
         }
-        pb[b][nt][0] = transpose8x8(pack_half2(e[0], e[1]));
-        pb[b][nt][1] = transpose8x8(pack_half2(e[2], e[3]));
-      }
+      l[nt][0] = sum.x;
+      l[nt][1] = sum.y;
     }
 #pragma unroll
     for (int b = 0; b < SUB; ++b) values(st, b, pb[b]);
   }
 
-  // This lane's key of the stage: its field and scales.
+  // This lane's key of the stage: its field and scales. With b' = beta log2(e), the bias plus lv of a row is b' min(a_s,
+  // M - psi_s) + lv, which times the sign of b' is min(a, low + e) for a = |b'| a_s + sign lv, e = -|b'| psi_s + sign lv
+  // and the row's low = |b'| M; sign f is the product's factor. No such key: a = e = -sign inf.
   struct Field {
     float phi, psi, f, lv, rv;
   };
@@ -430,6 +436,8 @@ struct MmaCore {
     later.values(c, job.h);
     sum_q();
     nw.low = prefix_min(nw.phi);
+    sign = job.bias < 0.f ? -1.f : 1.f;
+    const float strength = fabsf(job.bias);
     if (job.last && history < kStages - 1) {
       // Few blocks: the newest tokens' block and the empty groups after it.
       for (int i = history; i < kStages - 1; ++i) {
@@ -444,13 +452,16 @@ struct MmaCore {
         m[nt][q] = -kInf;
         l[nt][q] = 0.f;
         const int r = nt * 8 + 2 * t + q;
+        float x;
         if constexpr (kPrefix) {
-          low[nt][q] = r < job.rows ? p.row_min[int64_t(job.h) * (p.B * p.n) + job.r0 + r] : kInf;
+          x = r < job.rows ? p.row_min[int64_t(job.h) * (p.B * p.n) + job.r0 + r] : kInf;
         } else {
           const int i = job.r0 + r - job.lead;
-          const float x = __shfl_sync(0xffffffffu, nw.low, i & 31);
-          low[nt][q] = i >= 0 && i < job.n_new ? x : kInf;
+          x = __shfl_sync(0xffffffffu, nw.low, i & 31);
+          if (i < 0 || i >= job.n_new) x = kInf;
         }
+        // strength 0: the bias is 0 whatever the minimum is (not 0 times infinity).
+        low[nt][q] = strength == 0.f ? 0.f : strength * x;
 #pragma unroll
         for (int j = 0; j < MT; ++j) o[j][nt][q] = o[j][nt][q + 2] = 0.f;
       }
@@ -464,34 +475,38 @@ struct MmaCore {
         fetch_new(c, ring + ((i + kStages - 1) % kStages) * kStage, nw);
       copy_commit();
       const uint32_t st = ring + (i % kStages) * kStage;
-      float z[SUB][NT][4], rv[SUB][2];
+      float s[SUB][NT][4], rv[SUB][2];
+      float2 z[SUB][NT][2];  // per key g, g + 8 of each 16: rows 2t and 2t + 1
 #pragma unroll
-      for (int sub = 0; sub < SUB; ++sub) scores(st, sub, z[sub]);
+      for (int sub = 0; sub < SUB; ++sub) scores(st, sub, s[sub]);
+      float2 ref[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        ref[nt] = make_float2(m[nt][0] == -kInf ? 0.f : -m[nt][0], m[nt][1] == -kInf ? 0.f : -m[nt][1]);
+      const float2 sign2 = make_float2(sign, sign);
       if (i < history) {
         const int tile = job.t1 - 1 - i;
         const Field f = field_of(p, st, lane < kKeys && tile * kKeys + lane < job.end);
         float all;
         const float suf = fminf(suffix_min(f.phi, all), mid);
         mid = fminf(mid, all);
-        if (lane < kKeys) {
-          par[lane] = make_float4(fminf(suf - f.psi, 0.f), f.psi, f.f, f.lv);
-          if (kInt8) rvs[lane] = f.rv;
-        }
+        if (lane < kKeys)
+          par[lane] = make_float4(fmaf(-strength, f.psi, sign * f.lv), fmaf(strength, fminf(suf - f.psi, 0.f), sign * f.lv),
+                                  sign * f.f, f.rv);
         __syncwarp();
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub)
 #pragma unroll
           for (int key = 0; key < 2; ++key) {
-            const int at = sub * 16 + key * 8 + g;
-            const float4 x = par[at];
-            rv[sub][key] = kInt8 ? rvs[at] : 1.f;
+            const float4 x = par[sub * 16 + key * 8 + g];
+            rv[sub][key] = x.w;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                float& zz = z[sub][nt][2 * key + q];
-                zz = fmaf(zz, x.z, fmaf(job.bias, fminf(x.x, low[nt][q] - x.y), x.w));
-              }
+            for (int nt = 0; nt < NT; ++nt) {
+              const float2 t2 = __fadd2_rn(make_float2(low[nt][0], low[nt][1]), make_float2(x.x, x.x));
+              const float2 b = make_float2(fminf(x.y, t2.x), fminf(x.y, t2.y));
+              const float2 zz = __ffma2_rn(make_float2(s[sub][nt][2 * key], s[sub][nt][2 * key + 1]), make_float2(x.z, x.z), b);
+              z[sub][nt][key] = __ffma2_rn(zz, sign2, ref[nt]);
+            }
           }
       } else {
         // The newest tokens among themselves: range minima pair by pair.
@@ -504,14 +519,16 @@ struct MmaCore {
             const float ff = __shfl_sync(0xffffffffu, f.f, j & 31), lv = __shfl_sync(0xffffffffu, f.lv, j & 31);
             rv[sub][key] = __shfl_sync(0xffffffffu, f.rv, j & 31);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+              float zz[2];
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 const int i_ = job.r0 + nt * 8 + 2 * t + q - job.lead;
                 const float b = new_pair(nw, j, i_);
-                float& zz = z[sub][nt][2 * key + q];
-                zz = j < job.n_new && j <= i_ ? fmaf(zz, ff, fmaf(job.bias, b, lv)) : -kInf;
+                zz[q] = j < job.n_new && j <= i_ ? fmaf(s[sub][nt][2 * key + q], ff, fmaf(job.bias, b, lv)) : -kInf;
               }
+              z[sub][nt][key] = __fadd2_rn(make_float2(zz[0], zz[1]), ref[nt]);
+            }
           }
       }
       accumulate(st, z, rv);
