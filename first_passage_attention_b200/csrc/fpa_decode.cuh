@@ -129,16 +129,17 @@ __device__ __forceinline__ NewTokens load_new(const CacheView& c, int pid, int h
   return t;
 }
 
-// min_{j<u<=i} phi_u - psi_j, clamped at 0, for the new tokens j < i (0 for j == i). Warp-collective; j and i are the
-// calling lane's own.
-__device__ __forceinline__ float new_pair(const NewTokens& t, int j, int i) {
+// The newest tokens' pairs: table[j * kMaxNew + i] = min(0, min_{j<u<=i} phi_u - psi_j) for j < i, 0 for j == i. Lane j
+// fills row j with a running minimum.
+__device__ __forceinline__ void fill_pairs(const NewTokens& t, float* table) {
+  const int lane = threadIdx.x & 31;
   float m = kInf;
-  for (int u = 1; u < t.nn; ++u) {
-    const float f = __shfl_sync(0xffffffffu, t.phi, u);
-    if (u > j && u <= i) m = fminf(m, f);
+  for (int i = 0; i < t.nn; ++i) {
+    const float f = __shfl_sync(0xffffffffu, t.phi, i);
+    if (i > lane) m = fminf(m, f);
+    if (lane < t.nn) table[lane * kMaxNew + i] = fminf(m - t.psi, 0.f);
   }
-  const float psi = __shfl_sync(0xffffffffu, t.psi, j & 31);
-  return j < i ? fminf(m - psi, 0.f) : 0.f;
+  __syncwarp();
 }
 
 // What one CTA works on.
@@ -312,24 +313,26 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
 
 // Grid and launch of one pass. chunks (prefix): CTAs that share the prefix.
 //
-// CTAs of four warps for each (sequence, head, row group): as many as make two rounds of CTAs on the GPU, up to the 8 of
-// a cluster, and at least a block for each warp. Fewer leave SMs unevenly loaded at the end, more pay the start-up
-// chain too often (64 units of 16383 tokens, fp16 D = 128: 3 CTAs each 82 us, 4 to 6 70-71, 8, which is two rounds, 68;
-// 768 units of up to 2048, int8 D = 64: 34.3 us with one, 38.7 with two).
+// CTAs of four warps for each (sequence, head, row group): 1, 2, 4 or 8 (a cluster), as many as run at once on the GPU. An
+// eighth of the places is left free, since clusters do not fill the SMs of a GPC exactly: 72 units of 400 tokens, fp16 D =
+// 128, three CTAs on an SM, take 8.3 us with 4 CTAs each, 14.2 with 6 (432 of 444 places), where some wait for a second
+// round. Twice as many where every warp then still has kManyBlocks blocks: a second round evens out long work (64 units
+// of 16383 tokens, 5 rows: 71 us with 4, 68 with 8).
 template <class Core>
 cudaError_t launch_decode_core(DecodeParams p, bool prefix, cudaStream_t s) {
   const int rows = prefix ? p.B * p.n : p.n;
   p.groups = (rows + Core::NQ - 1) / Core::NQ;
-  const int by_regs = Core::kMinBlocks * kMaxWarps, by_smem = (227 * 1024) / decode_smem_bytes<Core>(1);
-  const int64_t slots = int64_t(sm_count()) * (by_regs < by_smem ? by_regs : by_smem);
   const int64_t units = int64_t(p.c.H) * p.groups * (prefix ? 1 : p.B);
   const int64_t len = prefix ? p.prefix_len : int64_t(p.max_pages) << p.c.page_shift;
   const int64_t blocks = (len + Core::kKeys - 1) / Core::kKeys;
-  int W = int(blocks < kMaxWarps ? blocks : kMaxWarps), splits = p.chunks;
+  const int W = int(blocks < kMaxWarps ? blocks : kMaxWarps);
+  int splits = prefix ? p.chunks : 1;
   if (!prefix) {
-    int64_t most = 2 * slots / (units * W);
-    if (most > blocks / W) most = blocks / W;
-    splits = int(most < 1 ? 1 : most > 8 ? 8 : most);
+    const int by_smem = (228 * 1024) / (decode_smem_bytes<Core>(W) + 1024);
+    const int64_t places = int64_t(sm_count()) * (by_smem < Core::kMinBlocks ? by_smem : Core::kMinBlocks);
+    while (splits < 8 && units * splits * 2 <= places * 7 / 8 && blocks >= int64_t(splits) * 2 * W) splits *= 2;
+    if (splits < 8 && units * splits <= places && blocks >= int64_t(splits) * 2 * W * Core::kManyBlocks)
+      splits *= 2;
   }
   const int smem = decode_smem_bytes<Core>(W);
   cudaLaunchConfig_t cfg = {};

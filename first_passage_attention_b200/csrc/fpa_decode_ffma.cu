@@ -3,69 +3,138 @@
 // A warp takes 32 keys at a time. Scores: lane (g, t) = (lane / 4, lane % 4) holds a quarter of key g of eight, in
 // runs of four elements that the four lanes of a key read side by side; two shuffles finish a product. The softmax has
 // one key per lane, and the product with V one run of D / 32 columns per lane, P coming from shared memory four keys
-// at a time. Everything is float32: this is the path of float32 models, whose tolerance rules out fp16 operands.
+// at a time. K and V come through a ring of the warp's own, eight rows to a stage, filled by cp.async kStages - 1 stages
+// ahead; rows are padded so that the lanes of a key and of its neighbour read different banks. Everything is float32:
+// this is the path of float32 models, whose tolerance rules out fp16 operands.
 #include "fpa_decode.cuh"
 
 namespace fpa {
 namespace {
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
 template <int D_, bool kInt8, int NR>
 struct FfmaCore {
-  static constexpr int D = D_, NQ = NR;
+  static constexpr int D = D_, NQ = NR, kKeys = 32;
   static constexpr int CPL = D < 32 ? 1 : D / 32;   // columns of V for a lane
-  static constexpr int CV = CPL < 4 ? CPL : 4;      // ... of one load
+  static constexpr int CV = CPL < 4 ? CPL : 4;      // ... side by side
   static constexpr int KG = D < 32 ? 32 / D : 1;    // lanes that share a column take every KG-th key
+  static constexpr int RB = kInt8 ? D : 4 * D;      // bytes of a row
+  static constexpr int kPitch = RB + (kInt8 ? 16 : D < 32 ? 0 : 64);
+  static constexpr int kStage = 8 * kPitch;         // eight rows of K or of V
+  static constexpr int kStages = kStage <= 2560 ? 6 : kStage <= 4608 ? 5 : 2;  // so that at least two CTAs fit an SM
+  static constexpr int kRingBytes = kStages * kStage;
   static constexpr int kMinBlocks = NR * CPL + D / 4 <= 64 ? 4 : 2;
-  static constexpr int kKeys = 32, kRingBytes = 0;
-  static constexpr int kCtaFloats = NR * D, kWarpFloats = NR * 32;
+  static constexpr int kCtaFloats = NR * D;
+  static constexpr int kScores = NR * 32, kSlots = 64;  // probabilities; the new tokens' pool indices (int64)
+  static constexpr int kWarpFloats = kScores + kSlots + kMaxNew * kMaxNew;
+  static constexpr int kManyBlocks = NR * D >= 512 ? 2 : 16;  // a block of many products outweighs a start-up sooner
   using Out = float;
+  static_assert(kStages <= 8, "at most one tile ahead");
 
   float o[NR][CPL], m[NR], l[NR];
-  float* qs;  // [NR][D]
-  float* ss;  // [NR][32], this warp's scores and probabilities
+  float* qs;         // [NR][D]
+  float* ss;         // [NR][32], this warp's scores and probabilities
+  int64_t* slots;    // [32]
+  float* pairs;      // [kMaxNew][kMaxNew]
+  char* ring_ptr;
+  uint32_t ring;
   int lane, g, t;
 
-  __device__ __forceinline__ FfmaCore(const DecodeParams&, const Job&, float* scratch, char*) {
+  __device__ __forceinline__ FfmaCore(const DecodeParams&, const Job&, float* scratch, char* rings) {
     lane = threadIdx.x & 31;
     g = lane >> 2;
     t = lane & 3;
     qs = scratch;
-    ss = scratch + NR * D + (threadIdx.x >> 5) * NR * 32;
+    ss = scratch + kCtaFloats + (threadIdx.x >> 5) * kWarpFloats;
+    slots = reinterpret_cast<int64_t*>(ss + kScores);
+    pairs = ss + kScores + kSlots;
+    ring_ptr = rings + (threadIdx.x >> 5) * kRingBytes;
+    ring = static_cast<uint32_t>(__cvta_generic_to_shared(ring_ptr));
   }
 
   __device__ __forceinline__ static int column(int j) { return (j / CV * 32 + (threadIdx.x & 31)) * CV + j % CV; }
 
-  // Four elements d .. d + 3 of the key at pool index `slot` (codes for int8).
-  __device__ __forceinline__ static float4 load4(const void* base, int64_t slot, int d) {
+  // Four elements d .. d + 3 of a row in shared memory (codes for int8).
+  __device__ __forceinline__ static float4 load4(const char* row, int d) {
     if constexpr (kInt8) {
-      const uchar4 x = __ldg(reinterpret_cast<const uchar4*>(static_cast<const char*>(base) + slot * D + d));
+      const uchar4 x = *reinterpret_cast<const uchar4*>(row + d);
       return make_float4(x.x - 128, x.y - 128, x.z - 128, x.w - 128);
     } else {
-      return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + slot * D + d));
+      return *reinterpret_cast<const float4*>(row + 4 * d);
     }
   }
 
-  // V of one key, this lane's columns.
-  __device__ __forceinline__ static void load_v(const void* base, int64_t slot, float (&v)[CPL]) {
+  // V of one row, this lane's columns.
+  __device__ __forceinline__ static void load_v(const char* row, float (&v)[CPL]) {
     if constexpr (CV == 4) {
 #pragma unroll
       for (int j = 0; j < CPL; j += 4) {
-        const float4 x = load4(base, slot, column(j));
+        const float4 x = load4(row, column(j));
         v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) {
-        const int64_t at = slot * D + (D < 32 ? (threadIdx.x & (D - 1)) : column(j));
-        v[j] = kInt8 ? float(__ldg(static_cast<const unsigned char*>(base) + at) - 128) : __ldg(static_cast<const float*>(base) + at);
+    } else if constexpr (CV == 2) {
+      const int d = column(0);
+      if constexpr (kInt8) {
+        const uchar2 x = *reinterpret_cast<const uchar2*>(row + d);
+        v[0] = x.x - 128, v[1] = x.y - 128;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(row + 4 * d);
+        v[0] = x.x, v[1] = x.y;
       }
+    } else {
+      const int d = threadIdx.x & (D < 32 ? D - 1 : 31);
+      v[0] = kInt8 ? float(static_cast<unsigned char>(row[d])) - 128.f : reinterpret_cast<const float*>(row)[d];
     }
   }
 
-  // Softmax of one key per lane (z = ss[r][lane] * f + bias(r) + lv) and the products with V of `n` keys whose pool
-  // indices are slot(0), slot(1), ...
-  template <class Bias, class Slot>
-  __device__ __forceinline__ void accumulate(const CacheView& c, float f, float lv, float rv, int n, Bias bias, Slot slot) {
+  // Eight rows into stage i: row r at pool index slot(r), zeros where that is negative.
+  template <class Slot>
+  __device__ __forceinline__ void fetch(const void* pool, int i, Slot slot) {
+    const uint32_t st = ring + (i % kStages) * kStage;
+    constexpr int kChunks = RB / 16;
+#pragma unroll
+    for (int e0 = 0; e0 < 8 * kChunks; e0 += 32) {
+      const int e = e0 + lane, r = e / kChunks, c = e % kChunks;
+      if (8 * kChunks < 32 && e >= 8 * kChunks) break;
+      const int64_t at = slot(r);
+      copy16(st + r * kPitch + c * 16, static_cast<const char*>(pool) + (at < 0 ? 0 : at) * RB + c * 16, at >= 0);
+    }
+  }
+
+  // Scores of the eight keys in stage i into columns first .. first + 7.
+  __device__ __forceinline__ void scores(int i, int first) {
+    const char* row = ring_ptr + (i % kStages) * kStage + g * kPitch;
+    float4 k[D / 16];
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) k[j] = load4(row, (j * 4 + t) * 4);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        const float4 q = *reinterpret_cast<const float4*>(qs + r * D + (j * 4 + t) * 4);
+        s = fmaf(q.x, k[j].x, s);
+        s = fmaf(q.y, k[j].y, s);
+        s = fmaf(q.z, k[j].z, s);
+        s = fmaf(q.w, k[j].w, s);
+      }
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (t == (r & 3)) ss[r * 32 + first + g] = s;
+    }
+  }
+
+  // Softmax of one key per lane: z = ss[r][lane] f + bias(r) + lv; no key where lv (or the bias) is -inf.
+  template <class Bias>
+  __device__ __forceinline__ void softmax(float f, float lv, float rv, Bias bias) {
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       const float b = bias(r);
@@ -84,30 +153,29 @@ struct FfmaCore {
       l[r] = fmaf(e, rv, l[r]);
       ss[r * 32 + lane] = e;
     }
-    __syncwarp();
+  }
+
+  // O += P V of the eight keys in stage i, columns first .. first + 7 of P.
+  __device__ __forceinline__ void values(int i, int first) {
+    const char* rows = ring_ptr + (i % kStages) * kStage;
     if constexpr (KG > 1) {
-      for (int k = lane / D; k < n; k += KG) {
-        const int64_t at = slot(k);
-        if (at < 0) continue;
-        float v[CPL];
-        load_v(c.v, at, v);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) o[r][0] = fmaf(ss[r * 32 + k], v[0], o[r][0]);
+      for (int k0 = 0; k0 < 8; k0 += KG) {
+        const int k = k0 + lane / D;
+        float v[CPL];
+        load_v(rows + k * kPitch, v);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) o[r][0] = fmaf(ss[r * 32 + first + k], v[0], o[r][0]);
       }
     } else {
-#pragma unroll 2
-      for (int k = 0; k < n; k += 4) {
+#pragma unroll
+      for (int k = 0; k < 8; k += 4) {
         float v[4][CPL];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t at = k + i < n ? slot(k + i) : -1;
-#pragma unroll
-          for (int j = 0; j < CPL; ++j) v[i][j] = 0.f;
-          if (at >= 0) load_v(c.v, at, v[i]);
-        }
+        for (int j = 0; j < 4; ++j) load_v(rows + (k + j) * kPitch, v[j]);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          const float4 e = *reinterpret_cast<const float4*>(ss + r * 32 + k);
+          const float4 e = *reinterpret_cast<const float4*>(ss + r * 32 + first + k);
 #pragma unroll
           for (int j = 0; j < CPL; ++j) {
             float x = o[r][j];
@@ -119,34 +187,54 @@ struct FfmaCore {
         }
       }
     }
-    __syncwarp();
-  }
-
-  // Scores of 8 keys (this lane's key g at pool index `at`, or -1) into columns first .. first + 7.
-  __device__ __forceinline__ void scores(const CacheView& c, int64_t at, int first) {
-    float4 k[D / 16];
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) k[j] = at >= 0 ? load4(c.k, at, (j * 4 + t) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        const float4 q = *reinterpret_cast<const float4*>(qs + r * D + (j * 4 + t) * 4);
-        s = fmaf(q.x, k[j].x, s);
-        s = fmaf(q.y, k[j].y, s);
-        s = fmaf(q.z, k[j].z, s);
-        s = fmaf(q.w, k[j].w, s);
-      }
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      if (t == (r & 3)) ss[r * 32 + first + g] = s;
-    }
   }
 
   template <bool kPrefix>
   __device__ __forceinline__ void run(const DecodeParams& p, const Job& job) {
     const CacheView& c = p.c;
+    // The run: history tiles from the latest to the earliest, then the newest tokens' tile. Stages 8 k .. 8 k + 3 hold
+    // K of tile k, 8 k + 4 .. 8 k + 7 its V, eight rows each.
+    const int history = job.t1 - job.t0, total = history + (job.last ? 1 : 0);
+    int64_t base = -1;   // of the tile being fetched
+    int lim = 0;
+    float phi = kInf, psi = 0.f, ks = 0.f, vs = 0.f;  // this lane's key of the tile being fetched
+    auto fetch_stage = [&](int i) {
+      const int tile = i >> 3, part = i & 7;
+      const void* pool = part < 4 ? c.k : c.v;
+      const int first = (part & 3) * 8;
+      if (tile < history) {
+        if (part == 0) {
+          const int at = (job.t1 - 1 - tile) * kKeys;
+          base = slot_of(c, job.table, job.h, at);
+          lim = base < 0 ? 0 : min(kKeys, job.end - at);
+          phi = kInf, psi = ks = vs = 0.f;
+          if (lane < lim) {
+            phi = c.phi[base + lane];
+            psi = c.psi[base + lane];
+            if (kInt8) {
+              ks = c.ks[base + lane];
+              vs = c.vs[base + lane];
+            }
+          }
+        }
+        fetch(pool, i, [&](int r) { return first + r < lim ? base + first + r : int64_t(-1); });
+      } else if (tile < total) {
+        fetch(pool, i, [&](int r) { return slots[first + r]; });
+      }
+    };
+    LaterMin later;
+    later.ids(c, job.table, job.t1 * kKeys, history > 0 ? job.end : 0);
+    NewTokens nw{kInf, 0.f, kInf, -1, 0};
+    if constexpr (!kPrefix)
+      nw = load_new(c, lane < job.n_new ? job.table[(job.end + lane) >> c.page_shift] : -1, job.h, job.end, job.n_new);
+    later.values(c, job.h);
+    slots[lane] = nw.slot;
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) {
+      fetch_stage(i);
+      copy_commit();
+    }
     for (int e = threadIdx.x; e < NR * D; e += blockDim.x) {
       const int r = e / D, d = e - r * D;
       float x = 0.f;
@@ -160,12 +248,9 @@ struct FfmaCore {
       }
       qs[e] = x;
     }
+    nw.low = prefix_min(nw.phi);
+    fill_pairs(nw, pairs);
     __syncthreads();
-    NewTokens nw{kInf, 0.f, kInf, -1, 0};
-    if constexpr (!kPrefix) {
-      nw = load_new(c, lane < job.n_new ? job.table[(job.end + lane) >> c.page_shift] : -1, job.h, job.end, job.n_new);
-      nw.low = prefix_min(nw.phi);
-    }
     float low[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
@@ -181,57 +266,58 @@ struct FfmaCore {
         low[r] = i >= 0 && i < job.n_new ? x : kInf;
       }
     }
-    if (job.t1 > job.t0) {
-      float mid = job.t1 * 32 < job.end ? later_min(c, job.table, job.h, job.t1 * 32, job.end) : kInf;
-      for (int tile = job.t1 - 1; tile >= job.t0; --tile) {
-        const int64_t base = slot_of(c, job.table, job.h, tile * 32);
-        const int lim = base < 0 ? 0 : min(32, job.end - tile * 32);
-        const bool ok = lane < lim;
-        const float phi = ok ? c.phi[base + lane] : kInf, psi = ok ? c.psi[base + lane] : 0.f;
-        float f = p.scale2, lv = ok ? 0.f : -kInf, rv = 1.f;
+    float mid = later.finish(c, job.table, job.h);
+    auto next = [&](int i) {
+      // Stage i has landed; the one before it is free for what comes kStages - 1 later.
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      fetch_stage(i + kStages - 1);
+      copy_commit();
+    };
+    for (int k = 0; k < total; ++k) {
+      // The tile's field, before the fetches go on to the next tile's.
+      const bool fresh = k >= history, ok = fresh ? nw.slot >= 0 : lane < lim;
+      float f_phi = phi, f_psi = psi, f_ks = ks, f_vs = vs;
+      if (fresh) {
+        f_ks = f_vs = 0.f;
         if (kInt8 && ok) {
-          const float v = fmaxf(c.vs[base + lane], 0x1p-90f);
-          f *= c.ks[base + lane];
-          lv = lg2(v);
-          rv = 1.f / v;
+          f_ks = c.ks[nw.slot];
+          f_vs = c.vs[nw.slot];
         }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        next(8 * k + j);
+        scores(8 * k + j, j * 8);
+      }
+      __syncwarp();
+      float f = p.scale2, lv = ok ? 0.f : -kInf, rv = 1.f;
+      if (kInt8 && ok) {
+        const float v = fmaxf(f_vs, 0x1p-90f);
+        f *= f_ks;
+        lv = lg2(v);
+        rv = 1.f / v;
+      }
+      if (!fresh) {
         float all;
-        const float suf = fminf(suffix_min(phi, all), mid);
+        const float suf = fminf(suffix_min(ok ? f_phi : kInf, all), mid);
         mid = fminf(mid, all);
-        const float a = fminf(suf - psi, 0.f);
+        const float a = fminf(suf - f_psi, 0.f);
+        softmax(f, lv, rv, [&](int r) { return ok ? job.bias * fminf(a, low[r] - f_psi) : 0.f; });
+      } else {
+        softmax(f, lv, rv, [&](int r) {
+          const int i = job.r0 + r - job.lead;
+          return lane <= i && i < job.n_new ? job.bias * pairs[lane * kMaxNew + i] : -kInf;
+        });
+      }
+      __syncwarp();
 #pragma unroll
-        for (int first = 0; first < 32; first += 8) scores(c, first + g < lim ? base + first + g : -1, first);
-        __syncwarp();
-        accumulate(
-            c, f, lv, rv, lim, [&](int r) { return ok ? job.bias * fminf(a, low[r] - psi) : 0.f; },
-            [&](int k) { return base + k; });
+      for (int j = 0; j < 4; ++j) {
+        next(8 * k + 4 + j);
+        values(8 * k + 4 + j, j * 8);
       }
     }
-    if constexpr (!kPrefix) {
-      if (job.last && job.n_new > 0) {
-#pragma unroll
-        for (int first = 0; first < 32; first += 8) {
-          const int64_t at = __shfl_sync(0xffffffffu, nw.slot, first + g);
-          scores(c, at, first);
-        }
-        __syncwarp();
-        float f = p.scale2, lv = nw.slot >= 0 ? 0.f : -kInf, rv = 1.f;
-        if (kInt8 && nw.slot >= 0) {
-          const float v = fmaxf(c.vs[nw.slot], 0x1p-90f);
-          f *= c.ks[nw.slot];
-          lv = lg2(v);
-          rv = 1.f / v;
-        }
-        accumulate(
-            c, f, lv, rv, job.n_new,
-            [&](int r) {
-              const int i = job.r0 + r - job.lead;
-              const float x = new_pair(nw, lane, i);
-              return lane <= i ? job.bias * x : -kInf;
-            },
-            [&](int k) { return slot_of(c, job.table, job.h, job.end + k); });
-      }
-    }
+    copy_wait<0>();
   }
 
   __device__ __forceinline__ void store(float* sm, float* sl, float* sO, int rows) {

@@ -98,8 +98,10 @@ struct MmaCore {
   // tokens, 5 rows: 64 us against 69); at D = 256 in fp16 few warps fit either way (48 us with three, 60 with two).
   static constexpr int kStages = RB < 512 ? 2 : 3;
   static constexpr int kRingBytes = kStages * kStage;   // of a warp
-  static constexpr int kCtaFloats = 0, kWarpFloats = kKeys * 4;
+  static constexpr int kCtaFloats = 0, kWarpFloats = kMaxNew * kMaxNew;  // keys' values, or the new pairs
+  static_assert(kWarpFloats >= kKeys * 4, "scratch");
   static constexpr int kMinBlocks = D * NT <= 64 ? (RB <= 64 ? 5 : 4) : D * NT <= 128 ? 3 : 2;
+  static constexpr int kManyBlocks = 16;  // of a warp: enough that a second round of CTAs pays its start-up
   using Out = __half;
 
   uint32_t qf[NT][KS][2];
@@ -509,8 +511,10 @@ struct MmaCore {
             }
           }
       } else {
-        // The newest tokens among themselves: range minima pair by pair.
+        // The newest tokens among themselves.
         const Field f = field_of(p, st, lane < kKeys && nw.slot >= 0);
+        float* pairs = reinterpret_cast<float*>(par);
+        fill_pairs(nw, pairs);
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub)
 #pragma unroll
@@ -524,8 +528,9 @@ struct MmaCore {
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 const int i_ = job.r0 + nt * 8 + 2 * t + q - job.lead;
-                const float b = new_pair(nw, j, i_);
-                zz[q] = j < job.n_new && j <= i_ ? fmaf(s[sub][nt][2 * key + q], ff, fmaf(job.bias, b, lv)) : -kInf;
+                zz[q] = -kInf;
+                if (j < job.n_new && j <= i_ && i_ < job.n_new)
+                  zz[q] = fmaf(s[sub][nt][2 * key + q], ff, fmaf(job.bias, pairs[j * kMaxNew + i_], lv));
               }
               z[sub][nt][key] = __fadd2_rn(make_float2(zz[0], zz[1]), ref[nt]);
             }
