@@ -399,6 +399,8 @@ extern "C" FPA_API int fpa_cache_append(const FpaAppendArgs* a, void* stream) {
   p.counts = a->counts;
   // n tokens touch at most this many pages, wherever they start.
   const dim3 grid(unsigned((int64_t(a->n) + 2 * c.page_size - 2) / c.page_size), c.H, a->B);
+  // 256 threads for a page's worth of tokens, 128 for a few: 32 x 12 (sequence, head) pairs of one token take 3.5 us with
+  // 128, 4.6 with 256; 16 x 12 of 64 tokens 7.7 and 6.8.
   const bool i8 = c.storage == FPA_STORE_I8;
   auto kernel = c.dtype == FPA_DTYPE_F16 ? (i8 ? append_kernel<__half, true> : append_kernel<__half, false>)
                                          : (i8 ? append_kernel<float, true> : append_kernel<float, false>);

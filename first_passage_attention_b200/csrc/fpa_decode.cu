@@ -12,10 +12,12 @@ int invalid(const char* msg) {
   return FPA_ERR_INVALID_ARGUMENT;
 }
 
-// The prefix pass runs on tcgen05 for fp16 queries with D = 64 or 128 and more than 16 rows in the batch; 16 rows or
-// fewer fit one pass of the mma.sync kernel over the prefix.
+// The prefix pass runs on tcgen05 for fp16 queries with D = 64 and more than 16 rows in the batch, or D = 128 and more
+// than 8; fewer fit one pass of the mma.sync kernel over the prefix. A whole call behind 8192 tokens, 12 heads, us with
+// mma.sync / tcgen05: int8 D = 64, 8 rows 13.5 / 17.3, 16 rows 16.5 / 17.6, 17 rows 22.8 / 17.8, 64 rows 30.8 / 21.2; fp16 D =
+// 128, 4 rows 16.1 / 17.5, 8 rows 18.2 / 17.9, 12 rows 26.9 / 18.2, 64 rows 58.5 / 27.7.
 bool prefix_on_tc(const FpaCache& c, int64_t rows) {
-  return c.dtype == FPA_DTYPE_F16 && (c.D == 64 || c.D == 128) && rows > 16;
+  return c.dtype == FPA_DTYPE_F16 && ((c.D == 64 && rows > 16) || (c.D == 128 && rows > 8));
 }
 
 // Parts of the prefix (CTAs that share a row group's or row tile's prefix). tcgen05: one CTA on every SM, two 128-key

@@ -631,6 +631,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   if (warp == kWarpMma) tmem_dealloc(tmem, 512);
 }
 
+// How often the rows stand in the 128 lanes: as often as they fit. Whole calls behind 8192 tokens, 12 heads, us with 4 / 2 /
+// 1 copies: int8 D = 64, 32 rows 18.6 / 19.3 / 21.6, 64 rows - / 21.1 / 22.9; fp16 D = 128, 32 rows 20.9 / 20.7 / 22.2.
 template <int D, bool kInt8>
 cudaError_t launch_rep(const DecodeParams& p, cudaStream_t s) {
   const int R = p.B * p.n;
