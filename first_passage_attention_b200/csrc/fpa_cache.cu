@@ -10,6 +10,7 @@
 // at a quarter of the rate. Stored is code + 128. A block of the append owns one page of one (sequence, head): it alone
 // writes the page's minimum of phi.
 #include "fpa_serve.h"
+#include "fpa_sm100.cuh"
 
 namespace fpa {
 namespace {
@@ -24,11 +25,14 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8], float top) {
   const float k = 127.f * rcp_approx_f(top);
   uint32_t w[8];
   float off = 0.f;  // largest distance from an integer
+  const float2 k2 = make_float2(k, k), round2 = make_float2(kRound, kRound), back2 = make_float2(-kRound, -kRound);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float c = __fmul_rn(x[j], k), r = __fadd_rn(c, kRound);
-    off = fmaxf(off, fabsf(__fsub_rn(c, __fsub_rn(r, kRound))));
-    w[j] = __float_as_uint(r);
+  for (int j = 0; j < 8; j += 2) {
+    const float2 c = __fmul2_rn(make_float2(x[j], x[j + 1]), k2), r = __fadd2_rn(c, round2);
+    const float2 i = __fadd2_rn(r, back2), d = __ffma2_rn(i, make_float2(-1.f, -1.f), c);
+    off = sm100::fmax3f(off, fabsf(d.x), fabsf(d.y));
+    w[j] = __float_as_uint(r.x);
+    w[j + 1] = __float_as_uint(r.y);
   }
   if (!(off < 0.5f - 0x1p-14f) || !(top < 0x1p100f)) {  // near a half, or the reciprocal leaves float32's normal range
 #pragma unroll

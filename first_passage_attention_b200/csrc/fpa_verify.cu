@@ -7,8 +7,8 @@
 // vocabulary is cut up.
 //
 // Bound by the bytes of three rows of V per sequence, and by latency when sequences are few: a cluster of CTAs shares a
-// sequence, every CTA finds `a` itself (a few gathers), takes a part of the vocabulary with eight entries' loads in
-// flight per thread, and leaves its best (score, index) in shared memory, which all compare through distributed shared
+// sequence, every CTA finds `a` itself (a few gathers), takes a part of the vocabulary, four entries to a load and
+// eight in flight per thread, and leaves its best (score, index) in shared memory, which all compare through distributed shared
 // memory. A thread divides only where w > 0.999 best e, without which w / e cannot reach its best so far. The target's
 // own scores are looked at in a second pass, in the rare case that the first finds nothing.
 #include "fpa_serve.h"
@@ -17,7 +17,7 @@ namespace fpa {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kAhead = 8;  // entries whose loads a thread has in flight
+constexpr int kAhead = 2;  // fours of entries whose loads a thread has in flight
 
 struct VerifyParams {
   const void* p;
@@ -35,42 +35,77 @@ struct VerifyParams {
   int n, V;
 };
 
-// Best score of the thread's entries v = first, first + step, ... of the row w = pr - qr (qr null: pr) over e, as a key:
-// scores are >= 0, so their bits order as they do; the complement of the index lets the lowest index win a tie.
+// The thread's best entry so far, as a key: scores are >= 0, so their bits order as they do; the complement of the index
+// lets the lowest index win a tie. Entries come with rising index, so a later one never wins a tie here.
+struct Best {
+  float score;
+  unsigned long long key;
+  __device__ __forceinline__ void take(float w, float n, int v) {
+    if (w > 0.f && !(w < score * n * 0.999f)) {
+      const float s = __fdiv_rn(w, n);
+      if (s > score || (key == 0 && s >= 0.f)) {
+        score = s;
+        key = (static_cast<unsigned long long>(__float_as_uint(s) + 1u) << 32) | (0xffffffffu - unsigned(v));
+      }
+    }
+  }
+};
+
+// Four consecutive entries, 16 or 8 bytes.
+__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+__device__ __forceinline__ void load4(const __half* p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+
+// Best of the row w = pr - qr (qr null: pr) over e; the thread is number `first` of `step`. Rows that start at multiples of
+// four entries' bytes are read four at a time, their last V % 4 entries by the first threads; others one at a time.
 template <typename T>
 __device__ __forceinline__ unsigned long long scan_row(const T* pr, const T* qr, const float* e, int V, int first, int step) {
-  float best = 0.f;
-  unsigned long long key = 0;
-  for (int v0 = first; v0 < V; v0 += kAhead * step) {
-    float w[kAhead], n[kAhead];
+  Best best{0.f, 0};
+  const uintptr_t at = reinterpret_cast<uintptr_t>(pr) | reinterpret_cast<uintptr_t>(qr);
+  int v0 = 0;
+  if (at % (4 * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(e) % 16 == 0) {
+    v0 = V & ~3;
+    for (int i0 = first * 4; i0 < v0; i0 += kAhead * step * 4) {
+      float w[kAhead][4], q[kAhead][4], n[kAhead][4];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int v = v0 + i * step;
+      for (int i = 0; i < kAhead; ++i) {
+        const int v = i0 + i * step * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[i][j] = q[i][j] = n[i][j] = 0.f;
+        if (v < v0) {
+          load4(pr + v, w[i]);
+          load4(e + v, n[i]);
+          if (qr) load4(qr + v, q[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) best.take(__fsub_rn(w[i][j], q[i][j]), n[i][j], i0 + i * step * 4 + j);
+    }
+  }
+  for (int i0 = v0 + first; i0 < V; i0 += 4 * kAhead * step) {
+    float w[4 * kAhead], n[4 * kAhead];
+#pragma unroll
+    for (int i = 0; i < 4 * kAhead; ++i) {
+      const int v = i0 + i * step;
       w[i] = n[i] = 0.f;
       if (v < V) {
         w[i] = to_f32(pr[v]);
         n[i] = e[v];
-      }
-    }
-    if (qr) {
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int v = v0 + i * step;
-        if (v < V) w[i] = __fsub_rn(w[i], to_f32(qr[v]));
+        if (qr) w[i] = __fsub_rn(w[i], to_f32(qr[v]));
       }
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (w[i] > 0.f && !(w[i] < best * n[i] * 0.999f)) {
-        const float score = __fdiv_rn(w[i], n[i]);
-        if (score > best || (key == 0 && score >= 0.f)) {  // a later index never wins a tie
-          best = score;
-          key = (static_cast<unsigned long long>(__float_as_uint(score) + 1u) << 32) | (0xffffffffu - unsigned(v0 + i * step));
-        }
-      }
-    }
+    for (int i = 0; i < 4 * kAhead; ++i) best.take(w[i], n[i], i0 + i * step);
   }
-  return key;
+  return best.key;
 }
 
 // Best key of the block, in every thread; `red` holds one key per warp.
