@@ -28,13 +28,14 @@ _HEAD_DIMS = (16, 32, 64, 128, 256)
 # The current stream's handle by device index, without building a Stream object (which costs as much as the launch).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _int32_on(name, x, index, shape):
+def _int32_on(name, x, index, n):
     if x.dtype != torch.int32 or x.get_device() != index:
         raise ValueError(f"{name} must be an int32 tensor on cuda:{index}")
-    if x.shape != shape or not x.is_contiguous():
-        raise ValueError(f"{name} must be contiguous with shape {tuple(shape)}")
+    if x.dim() != 1 or x.numel() != n or not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with shape ({n},)")
     return x.data_ptr()
 
 
@@ -48,7 +49,7 @@ def _table_on(x, index, B):
 
 
 def _call(fn, args, index):
-    if torch.cuda.current_device() == index:
+    if _device() == index:
         rc = fn(ctypes.byref(args), _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -133,7 +134,7 @@ class FPACache:
         _lib.APPEND_PACKER.pack_into(
             a, 0, self._addr, B, n, k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), phi.data_ptr(), *phi.stride(),
             psi.data_ptr(), *psi.stride(), *_table_on(block_table, dev, B),
-            _int32_on("start", start, dev, (B,)), 0 if counts is None else _int32_on("counts", counts, dev, (B,)))
+            _int32_on("start", start, dev, B), 0 if counts is None else _int32_on("counts", counts, dev, B))
         _call(lib.fpa_cache_append, a, dev)
         LaunchStats.kernels += 1
 
@@ -145,8 +146,8 @@ class FPACache:
         if n < 0:
             raise ValueError("n must not be negative")
         table = _table_on(block_table, dev, B)
-        start = 0 if start is None else _int32_on("start", start, dev, (B,))
-        lengths = 0 if lengths is None else _int32_on("lengths", lengths, dev, (B,))
+        start = 0 if start is None else _int32_on("start", start, dev, B)
+        lengths = 0 if lengths is None else _int32_on("lengths", lengths, dev, B)
         k = _empty((B, H, n, D), self.dtype, self.device)
         v = torch.empty_like(k)
         phi = torch.empty_strided((B, H, n), (H * n, n, 1), dtype=torch.float32, device=self.device)
@@ -192,14 +193,14 @@ def first_passage_decode(q, cache, block_table, lengths, beta, prefix_table=None
         raise ValueError("prefix_len must not be negative, and needs a prefix_table")
     if prefix_len > 0:
         pages = prefix_table.numel()
-        ptable = _int32_on("prefix_table", prefix_table, dev, (pages,))
+        ptable = _int32_on("prefix_table", prefix_table, dev, pages)
         if pages * cache.page_size < prefix_len:
             raise ValueError("the prefix is longer than the pages of its table")
-    o = _empty((B, H, n, D), q.dtype, cache.device)
+    o = torch.empty_like(q) if q.is_contiguous() else _empty((B, H, n, D), q.dtype, cache.device)
     if B == 0:
         return o
     table = _table_on(block_table, dev, B)
-    lengths = _int32_on("lengths", lengths, dev, (B,))
+    lengths = _int32_on("lengths", lengths, dev, B)
     ws, ws_ptr, nbytes = None, 0, 0
     if prefix_len > 0:
         with _on_device(cache.device):
@@ -226,10 +227,12 @@ def verify_draft(p, q, draft, u, noise, draft_lens=None):
     noise (a draw from the normalised residual), or argmax_v p_a / noise where every draft was accepted or the residual
     is nowhere positive; ties go to the lowest index. The tokens then have the target's distribution."""
     lib = _lib.load()
-    if p.dim() != 3 or q.dim() != 3 or q.shape[0] != p.shape[0] or q.shape[2] != p.shape[2] or p.shape[1] != q.shape[1] + 1:
+    ps, qs = p.shape, q.shape
+    if len(ps) != 3 or len(qs) != 3 or ps[0] != qs[0] or ps[1] != qs[1] + 1 or ps[2] != qs[2]:
         raise ValueError("p must have shape (B, n + 1, V) and q shape (B, n, V)")
-    B, n, V = q.shape
-    if p.dtype not in (torch.float16, torch.float32) or q.dtype != p.dtype:
+    B, n, V = qs
+    dt = p.dtype
+    if dt not in (torch.float16, torch.float32) or q.dtype != dt:
         raise ValueError("p and q must both be fp16 or both fp32")
     if draft.shape != (B, n) or draft.dtype != torch.int64:
         raise ValueError("draft must be an int64 tensor of shape (B, n)")
@@ -242,18 +245,20 @@ def verify_draft(p, q, draft, u, noise, draft_lens=None):
     dev = p.get_device()
     if dev < 0 or q.get_device() != dev or draft.get_device() != dev or u.get_device() != dev or noise.get_device() != dev:
         raise ValueError("p, q, draft, u and noise must be on one CUDA device")
-    if p.stride(2) != 1 or q.stride(2) != 1 or noise.stride(1) != 1:
+    sp, sq, sn = p.stride(), q.stride(), noise.stride()
+    if sp[2] != 1 or sq[2] != 1 or sn[1] != 1:
         p, q, noise = (x if x.stride(-1) == 1 else x.contiguous() for x in (p, q, noise))
-    lens = 0 if draft_lens is None else _int32_on("draft_lens", draft_lens, dev, (B,))
+        sp, sq, sn = p.stride(), q.stride(), noise.stride()
+    lens = 0 if draft_lens is None else _int32_on("draft_lens", draft_lens, dev, B)
     accepted = torch.empty_strided((B,), (1,), dtype=torch.int32, device=p.device)
     tokens = torch.empty_strided((B, n + 1), (n + 1, 1), dtype=torch.int64, device=p.device)
     if B == 0:
         return accepted, tokens
     a = _lib.FpaVerifyArgs()
     _lib.VERIFY_PACKER.pack_into(
-        a, 0, _lib.DTYPE_F16 if p.dtype == torch.float16 else _lib.DTYPE_F32, B, n, V, p.data_ptr(), *p.stride()[:2],
-        q.data_ptr(), *q.stride()[:2], draft.data_ptr(), *draft.stride(), u.data_ptr(), *u.stride(), noise.data_ptr(),
-        noise.stride(0), lens, accepted.data_ptr(), tokens.data_ptr())
+        a, 0, _lib.DTYPE_F16 if dt == torch.float16 else _lib.DTYPE_F32, B, n, V, p.data_ptr(), sp[0], sp[1], q.data_ptr(),
+        sq[0], sq[1], draft.data_ptr(), *draft.stride(), u.data_ptr(), *u.stride(), noise.data_ptr(), sn[0], lens,
+        accepted.data_ptr(), tokens.data_ptr())
     _call(lib.fpa_verify, a, dev)
     LaunchStats.kernels += 1
     return accepted, tokens
