@@ -17,7 +17,7 @@
 // distributed shared memory: one launch, no atomics, a fixed order.
 //
 // On a B200, whole calls in a graph: 4 x 16 pairs of 16383 fp16 tokens of 128, 5 rows, 64 us, 5.5 TB/s; 64 x 12 of up to 2048
-// tokens of 64, one row, fp16 43 us, 6.1 TB/s, int8 32 us, 4.6 TB/s; 12 heads of 1000 fp16 tokens 6.7 us; float32, 8 x 8 of
+// tokens of 64, one row, fp16 36 us, int8 33 us, 4.4 TB/s; 12 heads of 1000 fp16 tokens 6.7 us; float32, 8 x 8 of
 // 1000 tokens of 32, 3 rows, 12.8 us.
 #pragma once
 
@@ -25,7 +25,8 @@
 
 namespace fpa {
 
-constexpr int kMaxWarps = 4;  // of a CTA
+constexpr int kMaxWarps = 4;     // of a CTA
+constexpr int kMinSorted = 16, kMaxSorted = 64;  // sequences that a launch puts in the order of their lengths
 
 // Index of slot `pos` of head h in the pool's [n_pages, H, page_size] arrays, given its page's id, or -1 where the id
 // lies outside the pool (recorded in the status word).
@@ -146,6 +147,36 @@ __device__ __forceinline__ void fill_pairs(const NewTokens& t, float* table) {
   __syncwarp();
 }
 
+// The sequence of rank r when the batch is ordered by falling length (to one part in 32 of cap; equal ones in the
+// batch's order), the same in every warp of the grid. The rank's length is found bit by bit, by counting.
+__device__ __forceinline__ int by_length(const int32_t* lengths, int B, int r, int cap) {
+  const int lane = threadIdx.x & 31;
+  const int shift = max(0, 27 - __clz(cap));
+  int x[kMaxSorted / 32];
+#pragma unroll
+  for (int i = 0; i < kMaxSorted / 32; ++i)
+    x[i] = i * 32 + lane < B ? min(max(lengths[i * 32 + lane], 0), cap) >> shift : -1;
+  int at = 0;  // largest value that more than r sequences reach
+#pragma unroll
+  for (int bit = 16; bit > 0; bit >>= 1) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kMaxSorted / 32; ++i) n += __popc(__ballot_sync(0xffffffffu, x[i] >= at + bit));
+    if (n > r) at += bit;
+  }
+#pragma unroll
+  for (int i = 0; i < kMaxSorted / 32; ++i) r -= __popc(__ballot_sync(0xffffffffu, x[i] > at));
+  int b = 0;
+#pragma unroll
+  for (int i = 0; i < kMaxSorted / 32; ++i) {
+    const unsigned m = __ballot_sync(0xffffffffu, x[i] == at);
+    const unsigned who = __ballot_sync(0xffffffffu, x[i] == at && __popc(m & ((1u << lane) - 1)) == r);
+    if (who) b = i * 32 + __ffs(who) - 1;
+    r -= __popc(m);
+  }
+  return __reduce_max_sync(0xffffffffu, b);  // the same in every lane, and known to be
+}
+
 // What one CTA works on.
 struct Job {
   const int32_t* table;
@@ -191,7 +222,8 @@ __host__ __device__ constexpr int decode_smem_bytes(int warps) {
 
 // Core: the arithmetic of one warp over a run of keys (see fpa_decode_mma.cu, fpa_decode_ffma.cu).
 // kPrefix: the rows (b, i) of the whole batch against the prefix, partial results to the workspace.
-template <class Core, bool kPrefix>
+// kSorted: the batch's sequences in the order of their lengths, the longest first.
+template <class Core, bool kPrefix, bool kSorted>
 __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) float smem[];
   constexpr int NQ = Core::NQ, D = Core::D;
@@ -225,9 +257,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
   } else {
     job.h = blockIdx.y / p.groups;
     job.r0 = (blockIdx.y - job.h * p.groups) * NQ;
-    job.b = blockIdx.z;
-    job.table = p.table + job.b * p.table_stride;
     const int cap = int(min(int64_t(p.max_pages) << p.c.page_shift, int64_t(INT32_MAX)));
+    job.b = kSorted ? by_length(p.lengths, p.B, blockIdx.z, cap) : blockIdx.z;
+    job.table = p.table + job.b * p.table_stride;
     int L = p.lengths[job.b];
     if (L < 0 || L > cap) {
       report_bad_page(p.c.status, kSiteDecode);
@@ -322,6 +354,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
 // 128, three CTAs on an SM, take 8.3 us with 4 CTAs each, 14.2 with 6 (432 of 444 places), where some wait for a second
 // round. Twice as many where every warp then still has kManyBlocks blocks: a second round evens out long work (64 units
 // of 16383 tokens, 5 rows: 71 us with 4, 68 with 8).
+//
+// Where the CTAs do not all run at once, the batch goes in the order of its lengths, so that the short sequences come last
+// (in the batch's order / sorted, lengths drawn evenly up to the given one): 64 x 12 pairs, 2048 tokens of 64, fp16 41.8 /
+// 36.2 us, int8 32.3 / 33.4 and 34.0 / 32.9 in two drawings; 48 x 16, 4096 of 128, int8 79 / 62; the own parts of 64 x 12, 512 of
+// 64, int8, behind a prefix 32.4 / 28.8 (whole call). Equal lengths pay for the search: 38.2 / 39.4 in fp16. Fewer than 16
+// sequences gain nothing (12 x 16, 8000 of 128, fp16, 5 rows: 84.3 / 85.3), and more than 64 little (100 x 8, 1500 of 64:
+// 24.6 / 23.9 when handed over in order).
 template <class Core>
 cudaError_t launch_decode_core(DecodeParams p, bool prefix, cudaStream_t s) {
   const int rows = prefix ? p.B * p.n : p.n;
@@ -331,12 +370,14 @@ cudaError_t launch_decode_core(DecodeParams p, bool prefix, cudaStream_t s) {
   const int64_t blocks = (len + Core::kKeys - 1) / Core::kKeys;
   const int W = int(blocks < kMaxWarps ? blocks : kMaxWarps);
   int splits = prefix ? p.chunks : 1;
+  bool sorted = false;
   if (!prefix) {
     const int by_smem = (228 * 1024) / (decode_smem_bytes<Core>(W) + 1024);
     const int64_t places = int64_t(sm_count()) * (by_smem < Core::kMinBlocks ? by_smem : Core::kMinBlocks);
     while (splits < 8 && units * splits * 2 <= places * 7 / 8 && blocks >= int64_t(splits) * 2 * W) splits *= 2;
     if (splits < 8 && units * splits <= places && blocks >= int64_t(splits) * 2 * W * Core::kManyBlocks)
       splits *= 2;
+    sorted = p.B >= kMinSorted && p.B <= kMaxSorted && units * splits > places;
   }
   const int smem = decode_smem_bytes<Core>(W);
   cudaLaunchConfig_t cfg = {};
@@ -355,7 +396,8 @@ cudaError_t launch_decode_core(DecodeParams p, bool prefix, cudaStream_t s) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
-  auto kernel = prefix ? decode_kernel<Core, true> : decode_kernel<Core, false>;
+  auto kernel = prefix ? decode_kernel<Core, true, false>
+                       : sorted ? decode_kernel<Core, false, true> : decode_kernel<Core, false, false>;
   if (smem > 48 * 1024) {
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;

@@ -252,6 +252,21 @@ def test_decode_row_counts(dtype, storage, n):
     run_decode([n, n + 1, n - 1, 40 + n], n, 3, 64, 32, dtype, storage, seed=n)
 
 
+@pytest.mark.parametrize("B,H,n,D,dtype,storage,P", [(64, 12, 1, 16, F16, I8, 0), (33, 24, 5, 64, F16, None, 0), (2, 400, 3, 16, F32, None, 0),
+                                                     (50, 24, 1, 64, F16, I8, 40), (65, 12, 2, 32, F16, I8, 0)])
+def test_decode_more_pairs_than_run_at_once(B, H, n, D, dtype, storage, P):
+    """The CTAs take the sequences in the order of their lengths: many equal ones, empty ones, the longest last."""
+    lens = [min(i * 37 % 150, 101) for i in range(B - 1)] + [160]
+    cache, table, qn, beta, got, kw = run_decode(lens, n, H, D, 32, dtype, storage, seed=B, P=P)
+    bad = list(lens)
+    bad[1] = table.shape[1] * 32 + 1  # beyond the table: the page ids there are -1, so nothing outside is read
+    bad[0] = -7
+    out = first_passage_decode(qn.cuda(), cache, table, i32(bad), beta.cuda(), **kw)
+    with pytest.raises(ValueError):
+        cache.check()
+    assert torch.equal(out[2:], got[2:])
+
+
 @pytest.mark.parametrize("beta", [-0.7, 0.0, 3.0])
 @pytest.mark.parametrize("dtype,storage", [(F16, I8), (F32, None)])
 def test_decode_beta_and_wide_fields(beta, dtype, storage):
