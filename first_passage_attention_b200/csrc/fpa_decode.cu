@@ -88,6 +88,7 @@ extern "C" FPA_API int fpa_decode(FpaDecodeArgs* a, void* stream) {
   const bool i8 = c.storage == FPA_STORE_I8, f16 = c.dtype == FPA_DTYPE_F16;
   auto run = f16 ? launch_decode_mma : launch_decode_ffma;
   cudaError_t e;
+  int launches = 0;
   if (p.prefix_len > 0) {
     size_t ml, o;
     const size_t need = workspace_bytes(c, p.B, p.n, p.prefix_len, &ml, &o);
@@ -104,21 +105,22 @@ extern "C" FPA_API int fpa_decode(FpaDecodeArgs* a, void* stream) {
     e = launch_row_min(p, s);
     if (e == cudaSuccess) {
       prof_mark(s, "decode_prefix");
-      e = prefix_on_tc(c, int64_t(p.B) * p.n) ? launch_prefix_tc(p, i8, s) : run(p, i8, true, s);
+      e = prefix_on_tc(c, int64_t(p.B) * p.n) ? launch_prefix_tc(p, i8, s) : run(p, i8, true, s, launches);
     }
     if (e != cudaSuccess) {
       set_last_error(std::string("fpa_decode, prefix: ") + cudaGetErrorString(e));
       return FPA_ERR_CUDA;
     }
     a->kernels_launched = 2;
+    launches = 0;
   }
   prof_mark(s, "decode");
-  e = run(p, i8, false, s);
+  e = run(p, i8, false, s, launches);
   prof_mark(s, nullptr);
   if (e != cudaSuccess) {
     set_last_error(std::string("fpa_decode: ") + cudaGetErrorString(e));
     return FPA_ERR_CUDA;
   }
-  a->kernels_launched += 1;
+  a->kernels_launched += launches;
   return FPA_OK;
 }

@@ -14,7 +14,7 @@
 // to the earliest, so that SUF is a running minimum that the warp carries in a register, and no warp waits for
 // another until the end. What lies after a warp's run enters through the page minima (phi_min), four bytes a page and
 // head. The softmax states (m, l, O) of the warps join in shared memory, those of the cluster's CTAs through
-// distributed shared memory: one launch, no atomics, a fixed order.
+// distributed shared memory: no atomics, a fixed order, one launch (two where a last round would stay mostly empty).
 //
 // On a B200, whole calls in a graph: 4 x 16 pairs of 16383 fp16 tokens of 128, 5 rows, 64 us, 5.5 TB/s; 64 x 12 of up to 2048
 // tokens of 64, one row, fp16 36 us, int8 33 us, 4.4 TB/s; 12 heads of 1000 fp16 tokens 6.7 us; float32, 8 x 8 of
@@ -238,11 +238,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
   const int S = gridDim.x, rank = blockIdx.x;
   // A prefix pass before this kernel has waited for everything before it, so only its own results are still open:
   // the wait then moves to where they are read.
-  const bool late = !kPrefix && p.prefix_len > 0;
-  if (!late) {
-    pdl_wait();
-    pdl_launch_dependents();
-  }
+  const bool behind = !kPrefix && p.prefix_len > 0;
+  // The same holds for a second launch behind the first one, which has waited too (or is late itself, behind a prefix
+  // pass that has); its wait at the end leaves whatever comes after this launch behind both.
+  const bool late = !kPrefix && (behind || p.follows);
+  if (!late) pdl_wait();
+  if (!late || p.followed) pdl_launch_dependents();
   Job job;
   int R = p.n;
   if constexpr (kPrefix) {
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
     job.h = blockIdx.y / p.groups;
     job.r0 = (blockIdx.y - job.h * p.groups) * NQ;
     const int cap = int(min(int64_t(p.max_pages) << p.c.page_shift, int64_t(INT32_MAX)));
-    job.b = kSorted ? by_length(p.lengths, p.B, blockIdx.z, cap) : blockIdx.z;
+    job.b = kSorted ? by_length(p.lengths, p.B, p.first + blockIdx.z, cap) : p.first + blockIdx.z;
     job.table = p.table + job.b * p.table_stride;
     int L = p.lengths[job.b];
     if (L < 0 || L > cap) {
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
       float M = -kInf;
       const int64_t pre = ((int64_t(job.h) * p.B + job.b) * p.n + row) * p.chunks;
       for (int c = 0; c < S; ++c) M = fmaxf(M, S > 1 ? cluster_ld(cluster_addr(cm + r, c)) : cm[r]);
-      if (late)
+      if (behind)
         for (int c = 0; c < p.chunks; ++c) M = fmaxf(M, p.part_ml[(pre + c) * 2]);
       float l = 0.f, o = 0.f;
       for (int c = 0; c < S; ++c) {
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
         l += w * (S > 1 ? cluster_ld(cluster_addr(cl + r, c)) : cl[r]);
         o += w * (S > 1 ? cluster_ld(cluster_addr(sO + e, c)) : sO[e]);
       }
-      if (late)
+      if (behind)
         for (int c = 0; c < p.chunks; ++c) {
           const float w = state_weight(p.part_ml[(pre + c) * 2], M);
           l += w * p.part_ml[(pre + c) * 2 + 1];
@@ -361,8 +362,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
 // 64, int8, behind a prefix 32.4 / 28.8 (whole call). Equal lengths pay for the search: 38.2 / 39.4 in fp16. Fewer than 16
 // sequences gain nothing (12 x 16, 8000 of 128, fp16, 5 rows: 84.3 / 85.3), and more than 64 little (100 x 8, 1500 of 64:
 // 24.6 / 23.9 when handed over in order).
+//
+// What a last, partly filled round holds goes in a launch of its own with up to four CTAs each, whose CTAs start as the
+// first launch's end (one launch / two; table as wide as the lengths): 64 x 12, 2048 int8 tokens of 64, all of them 52.9 /
+// 45.6 us, uneven 31.3 / 29.4; 40 x 12 in fp16 55.0 / 47.5 and 25.1 / 26.8; 28 x 16 of 128, fp16, 5 rows, 97 / 84 and 48.1 / 49.8. Not
+// for short runs (64 x 12 of 512: 19.8 / 19.5 and 12.5 / 14.3) or many rounds (130 x 12: 87 / 79 and 48 / 51).
 template <class Core>
-cudaError_t launch_decode_core(DecodeParams p, bool prefix, cudaStream_t s) {
+cudaError_t launch_decode_core(DecodeParams p, bool prefix, cudaStream_t s, int& launches) {
   const int rows = prefix ? p.B * p.n : p.n;
   p.groups = (rows + Core::NQ - 1) / Core::NQ;
   const int64_t units = int64_t(p.c.H) * p.groups * (prefix ? 1 : p.B);
@@ -371,6 +377,7 @@ cudaError_t launch_decode_core(DecodeParams p, bool prefix, cudaStream_t s) {
   const int W = int(blocks < kMaxWarps ? blocks : kMaxWarps);
   int splits = prefix ? p.chunks : 1;
   bool sorted = false;
+  int rest = 0, rest_splits = 0;
   if (!prefix) {
     const int by_smem = (228 * 1024) / (decode_smem_bytes<Core>(W) + 1024);
     const int64_t places = int64_t(sm_count()) * (by_smem < Core::kMinBlocks ? by_smem : Core::kMinBlocks);
@@ -378,31 +385,52 @@ cudaError_t launch_decode_core(DecodeParams p, bool prefix, cudaStream_t s) {
     if (splits < 8 && units * splits <= places && blocks >= int64_t(splits) * 2 * W * Core::kManyBlocks)
       splits *= 2;
     sorted = p.B >= kMinSorted && p.B <= kMaxSorted && units * splits > places;
+    const int64_t each = int64_t(p.c.H) * p.groups, round = places / (each * splits);
+    if (round > 0 && p.B > round && p.B <= kMaxSorted && blocks >= int64_t(splits) * W * 8) {
+      rest = int(p.B % round);
+      rest_splits = splits;
+      while (rest_splits < 4 && each * rest * rest_splits * 2 <= places * 7 / 8) rest_splits *= 2;
+      if (rest_splits == splits) rest = 0;
+    }
   }
   const int smem = decode_smem_bytes<Core>(W);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = prefix ? dim3(splits, p.groups, p.c.H) : dim3(splits, p.c.H * p.groups, p.B);
-  cfg.blockDim = dim3(W * 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (!prefix && splits > 1) {
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = splits;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.numAttrs = 2;
-  }
   auto kernel = prefix ? decode_kernel<Core, true, false>
                        : sorted ? decode_kernel<Core, false, true> : decode_kernel<Core, false, false>;
   if (smem > 48 * 1024) {
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
   }
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  auto launch = [&](int count, int splits_) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = prefix ? dim3(splits_, p.groups, p.c.H) : dim3(splits_, p.c.H * p.groups, count);
+    cfg.blockDim = dim3(W * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (!prefix && splits_ > 1) {
+      attr[1].id = cudaLaunchAttributeClusterDimension;
+      attr[1].val.clusterDim.x = splits_;
+      attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+      cfg.numAttrs = 2;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    launches += e == cudaSuccess;
+    return e;
+  };
+  if (rest > 0) {
+    p.followed = true;
+    const cudaError_t e = launch(p.B - rest, splits);
+    if (e != cudaSuccess) return e;
+    p.first = p.B - rest;
+    p.followed = false;
+    p.follows = true;
+    return launch(rest, rest_splits);
+  }
+  return launch(p.B, splits);
 }
 
 }  // namespace fpa

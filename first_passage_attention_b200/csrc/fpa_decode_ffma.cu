@@ -346,15 +346,15 @@ struct FfmaCore {
 // us for groups of 1 / 4 / 8: 8 rows, D = 32 int8 84 / 41 / 38, D = 64 147 / 88 / 87, D = 128 246 / 134 / 135; 2000 tokens at D =
 // 256 200 / 100 / 127 (the registers of 8 rows leave fewer CTAs); 2 rows, D = 32 29 / 25 / 37.
 template <bool kInt8>
-cudaError_t launch_for(const DecodeParams& p, bool prefix, cudaStream_t s) {
+cudaError_t launch_for(const DecodeParams& p, bool prefix, cudaStream_t s, int& launches) {
   const int rows = prefix ? p.B * p.n : p.n;
   switch (p.c.D) {
 #define FPA_CASE(D)                                                                                \
   case D:                                                                                          \
-    return rows == 1 ? launch_decode_core<FfmaCore<D, kInt8, 1>>(p, prefix, s)                     \
+    return rows == 1 ? launch_decode_core<FfmaCore<D, kInt8, 1>>(p, prefix, s, launches)                     \
            : rows < 5 || D > 64                                                                    \
-               ? launch_decode_core<FfmaCore<D, kInt8, 4>>(p, prefix, s)                           \
-               : launch_decode_core<FfmaCore<D, kInt8, D <= 64 ? 8 : 4>>(p, prefix, s);
+               ? launch_decode_core<FfmaCore<D, kInt8, 4>>(p, prefix, s, launches)                           \
+               : launch_decode_core<FfmaCore<D, kInt8, D <= 64 ? 8 : 4>>(p, prefix, s, launches);
     FPA_CASE(16)
     FPA_CASE(32)
     FPA_CASE(64)
@@ -392,8 +392,8 @@ __global__ void __launch_bounds__(128) row_min_kernel(const __grid_constant__ De
 
 }  // namespace
 
-cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s) {
-  return int8 ? launch_for<true>(p, prefix, s) : launch_for<false>(p, prefix, s);
+cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s, int& launches) {
+  return int8 ? launch_for<true>(p, prefix, s, launches) : launch_for<false>(p, prefix, s, launches);
 }
 
 cudaError_t launch_row_min(const DecodeParams& p, cudaStream_t s) {

@@ -568,7 +568,7 @@ struct MmaCore {
 };
 
 template <bool kInt8>
-cudaError_t launch_for(const DecodeParams& p, bool prefix, cudaStream_t s) {
+cudaError_t launch_for(const DecodeParams& p, bool prefix, cudaStream_t s, int& launches) {
   // 16 rows at a time where there are more than 8, so that the keys are read and converted once: 16 x 12 (sequence, head)
   // pairs of 4096 int8 tokens, D = 64, 16 rows 34 us against 52 in two groups of 8; 4 x 16 of 16383, fp16 D = 128 106 against
   // 146 (short calls differ by little: 72 pairs of 1000 tokens 12.7 against 11.5). Not at D = 256, whose accumulators
@@ -577,22 +577,22 @@ cudaError_t launch_for(const DecodeParams& p, bool prefix, cudaStream_t s) {
   switch (p.c.D) {
 #define FPA_CASE(D)                                                                            \
   case D:                                                                                      \
-    return wide ? launch_decode_core<MmaCore<D, kInt8, 2>>(p, prefix, s)               \
-                : launch_decode_core<MmaCore<D, kInt8, 1>>(p, prefix, s);
+    return wide ? launch_decode_core<MmaCore<D, kInt8, 2>>(p, prefix, s, launches)               \
+                : launch_decode_core<MmaCore<D, kInt8, 1>>(p, prefix, s, launches);
     FPA_CASE(16)
     FPA_CASE(32)
     FPA_CASE(64)
     FPA_CASE(128)
 #undef FPA_CASE
     default:
-      return launch_decode_core<MmaCore<256, kInt8, 1>>(p, prefix, s);
+      return launch_decode_core<MmaCore<256, kInt8, 1>>(p, prefix, s, launches);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s) {
-  return int8 ? launch_for<true>(p, prefix, s) : launch_for<false>(p, prefix, s);
+cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s, int& launches) {
+  return int8 ? launch_for<true>(p, prefix, s, launches) : launch_for<false>(p, prefix, s, launches);
 }
 
 }  // namespace fpa

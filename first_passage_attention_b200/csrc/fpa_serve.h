@@ -59,11 +59,14 @@ struct DecodeParams {
   float* part_ml;  // [H][R][chunks][2]  softmax maximum and sum of each chunk of the prefix
   float* part_o;   // [H][R][chunks][D]  unnormalised output of each chunk
   int chunks;
+  // The batch in two launches: the sequences from `first` on; another launch follows; another one went before.
+  int first;
+  bool followed, follows;
 };
 
 // Rows are handled by one CTA in groups of 8 or 16 (tensor cores) or 1, 4 or 8 (FFMA).
-cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s);
-cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s);
+cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s, int& launches);
+cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s, int& launches);
 // The prefix on tcgen05: fp16 queries, D = 64 or 128. p.chunks: CTAs that share a row tile's prefix.
 int prefix_tc_row_tiles(int64_t rows);
 cudaError_t launch_prefix_tc(const DecodeParams& p, bool int8, cudaStream_t s);

@@ -267,6 +267,32 @@ def test_decode_more_pairs_than_run_at_once(B, H, n, D, dtype, storage, P):
     assert torch.equal(out[2:], got[2:])
 
 
+@pytest.mark.parametrize("B,H,n,D,dtype,storage,P", [(64, 12, 1, 16, F16, I8, 0), (40, 12, 3, 64, F16, None, 0), (64, 12, 1, 32, F16, I8, 50),
+                                                     (15, 64, 2, 64, F16, I8, 0), (62, 16, 1, 32, F32, None, 0)])
+def test_decode_in_two_launches(B, H, n, D, dtype, storage, P):
+    """Long tables, a few sequences more than one round of CTAs holds. What follows on the stream waits for both."""
+    lens = [min(i * 37 % 150, 101) for i in range(B - 3)] + [1030, 3, 640]
+    cache, table, qn, beta, got, kw = run_decode(lens, n, H, D, 64, dtype, storage, seed=B, P=P)
+    q, lengths, beta = qn.cuda(), i32(lens), beta.cuda()
+    LaunchStats.reset()
+    assert torch.equal(first_passage_decode(q, cache, table, lengths, beta, **kw), got)
+    assert LaunchStats.kernels == (4 if P else 2) or dtype == F32
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = first_passage_decode(q, cache, table, lengths, beta, **kw)
+    graph.replay()
+    assert torch.equal(out, got)
+    # Calls in a row, the newest token rewritten before each: every call sees its own.
+    last = i32([max(x - 1, 0) for x in lens])
+    _, k, v, phi, psi = (x.cuda() for x in sequence(B, H, 2, D, dtype, seed=9))
+    outs = [[], []]
+    for i in range(20):
+        j = i & 1
+        cache.append(k[:, :, j:j + 1], v[:, :, j:j + 1], phi[..., j:j + 1], psi[..., j:j + 1], table, last, (lengths > 0).int())
+        outs[j].append(first_passage_decode(q, cache, table, lengths, beta, **kw))
+    assert all(torch.equal(x, y[0]) for y in outs for x in y) and not torch.equal(outs[0][0], outs[1][0])
+
+
 @pytest.mark.parametrize("beta", [-0.7, 0.0, 3.0])
 @pytest.mark.parametrize("dtype,storage", [(F16, I8), (F32, None)])
 def test_decode_beta_and_wide_fields(beta, dtype, storage):
