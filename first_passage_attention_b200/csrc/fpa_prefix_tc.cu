@@ -3,8 +3,8 @@
 // The rows (b, i) of all sequences, up to 128 at a time, meet every key of the prefix once: S = Q K^T and O += P V with
 // 128-key tiles, one CTA on an SM for a part of the prefix, which it walks from the latest tile to the earliest (the
 // mathematics is in fpa_decode.cuh). With R rows there are R flops a byte in fp16 and 2 R in int8, so for few rows the
-// prefix's bytes bound it; at 128 rows and D = 128 a tile takes 1024 cycles of MMAs, as many of exponentials, and as
-// many to bring its 64 KB to the SM. Where the rows fill half or a quarter of the 128 lanes, they stand there twice or
+// prefix's bytes bound it; at 128 rows and D = 128 a tile takes 1024 cycles of MMAs, as many of exponentials, and its
+// 64 KB take 2.8k cycles at an SM's share of the HBM rate (1024 from L2). Where the rows fill half or a quarter of the 128 lanes, they stand there twice or
 // four times, and each copy takes its half or quarter of the tile's keys (its P stays zero for the others), so that no
 // warp idles; the copies' softmax states join at the end.
 //
