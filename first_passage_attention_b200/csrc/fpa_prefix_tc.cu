@@ -42,6 +42,10 @@ struct PrefixCfg {
   static constexpr int BOXB = kTile * 128;                // a tile's 64 columns
   static constexpr int TILEB = D / 64 * BOXB;             // K or V of a tile in fp16
   static constexpr int SLOTS = kInt8 ? (D == 64 ? 6 : 3) : (D == 64 ? 8 : 5);
+  // Barriers that a unit's slot is free again: one for each slot and kind (K, V) that stands there. With an odd number
+  // of slots both kinds take turns in a slot, and a loader, which only waits for the unit before its own, would miss every
+  // other phase of a barrier that they shared: V of tile k could then pass before V of tile k - 3 has been read.
+  static constexpr int EMPTIES = SLOTS % 2 ? 2 * SLOTS : SLOTS;
   static constexpr int RAWB = kInt8 ? kTile * D : 0;      // K or V of a tile in codes
   static constexpr int RAWS = kInt8 ? (D == 64 ? 3 : 2) : 0;  // of K, and as many of V
   static constexpr int PARF = kInt8 ? 8 : 4;              // floats of a pair of keys
@@ -52,7 +56,7 @@ struct PrefixCfg {
   static constexpr int OFF_PAR = OFF_RAW + 2 * RAWS * RAWB;
   static constexpr int OFF_ML = OFF_PAR + kParStages * PARB;  // the states' maxima and sums [2][256]
   static constexpr int OFF_BAR = OFF_ML + 512 * 4;
-  static constexpr int NBAR = 2 * SLOTS + 2 * kParStages + 10;
+  static constexpr int NBAR = SLOTS + EMPTIES + 2 * kParStages + 10;
   static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
   static constexpr int COL_S = 0, COL_O = 2 * kTile;  // S of tile k: + 128 (k & 1), of group g: + 64 g; O: + D g
   static constexpr uint32_t IDESC_S = idesc_f16(kTile, kTile, 0);
@@ -102,7 +106,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* empty = full + C::SLOTS;
-  uint64_t* par_full = empty + C::SLOTS;
+  uint64_t* par_full = empty + C::EMPTIES;
   uint64_t* par_empty = par_full + kParStages;
   uint64_t* s_full = par_empty + kParStages;
   uint64_t* p_full = s_full + 2;
@@ -122,10 +126,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   const int nt = each + (int(blockIdx.x) < more ? 1 : 0), t1 = t0 + nt;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::SLOTS; ++i) {
-      mbar_init(full + i, kLoaders);
-      mbar_init(empty + i, 1);
-    }
+    for (int i = 0; i < C::SLOTS; ++i) mbar_init(full + i, kLoaders);
+    for (int i = 0; i < C::EMPTIES; ++i) mbar_init(empty + i, 1);
     for (int i = 0; i < kParStages; ++i) {
       mbar_init(par_full + i, 32);
       mbar_init(par_empty + i, 256);
@@ -220,7 +222,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
           cp_commit();
           cp_wait<C::RAWS - 1>();
           const int u = 2 * k + kv, slot = u % C::SLOTS;
-          if (u >= C::SLOTS) ok = mbar_wait(empty + slot, ((u / C::SLOTS) - 1) & 1, c.status, 71);
+          const int before = u - C::SLOTS;  // the unit whose place this one takes
+          if (before >= 0) ok = mbar_wait(empty + before % C::EMPTIES, (before / C::EMPTIES) & 1, c.status, 71);
           if (!ok) break;
           const uint32_t from = raw + (k % C::RAWS) * C::RAWB, to = ring + slot * C::TILEB;
           const uint32_t to_a = to + tile_chunk(row0, 2 * ch), to_b = to + tile_chunk(row0, 2 * ch + 1);
@@ -251,15 +254,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         for (int k = 0; k < nt; ++k) {
           const int u = 2 * k + kv, slot = u % C::SLOTS;
           if (u >= C::SLOTS) {
-            const uint32_t parity = ((u / C::SLOTS) - 1) & 1;
-            while (handed < k && !__all_sync(0xffffffffu, mbar_test_wait(empty + slot, parity))) {
+            const int before = u - C::SLOTS;  // the unit whose place this one takes
+            uint64_t* const freed = empty + before % C::EMPTIES;
+            const uint32_t parity = (before / C::EMPTIES) & 1;
+            while (handed < k && !__all_sync(0xffffffffu, mbar_test_wait(freed, parity))) {
               if (k - handed > 1 && kAhead > 1)
                 cp_wait<1>();  // all but the youngest
               else
                 cp_wait<0>();
               hand_over();
             }
-            ok = mbar_wait(empty + slot, parity, c.status, 72);
+            ok = mbar_wait(freed, parity, c.status, 72);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
           }
@@ -291,7 +296,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
             mma_ss(tmem + C::COL_S + (k & 1) * kTile, desc_make(lq + off, HI), desc_make(lb + off, HI), C::IDESC_S, kk > 0);
           }
           mma_commit(s_full + (k & 1));
-          mma_commit(empty + slot);
+          mma_commit(empty + (2 * k) % C::EMPTIES);
         }
         __syncwarp();
       };
@@ -304,7 +309,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
             mma_ts(tmem + C::COL_O + g * D, tmem + C::COL_S + (k & 1) * kTile + g * 64 + kk * 8,
                    desc_make(lb + uint32_t((kk * 16 * 128) >> 4), HI), C::IDESC_O, (k > 0 || kk > 0) ? 1u : 0u);
           mma_commit(o_ready + g);
-          if (g == 1) mma_commit(empty + slot);
+          if (g == 1) mma_commit(empty + (2 * k + 1) % C::EMPTIES);
         }
         __syncwarp();
       };

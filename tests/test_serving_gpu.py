@@ -322,6 +322,20 @@ def test_prefix_on_the_tensor_cores(D, storage, B, n, P, page):
     run_decode([(11 * b) % 50 for b in range(B)], n, 2, D, page, F16, storage, seed=B + P, P=P)
 
 
+@pytest.mark.parametrize("B,n", [(3, 4), (6, 9), (9, 10)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("storage", [None, I8])
+def test_prefix_ahead_of_the_rows_minima(D, storage, B, n):
+    """Four and more tiles of the prefix in a CTA, and long own histories in small pages: the rows' minima come late, so
+    the loads run as far ahead as the ring lets them. Many calls in a row give the same bits."""
+    lens = [2000 - 100 * b for b in range(B)]
+    cache, table, qn, beta, got, kw = run_decode(lens, n, 9, D, 32, F16, storage, seed=B, P=7345)
+    q, beta = qn.cuda(), beta.cuda()
+    for _ in range(50):
+        assert torch.equal(first_passage_decode(q, cache, table, i32(lens), beta, **kw), got)
+    cache.check()
+
+
 def test_prefix_rows_far_apart():
     """Rows whose scores differ by thousands beside ordinary ones, and a falling field: maxima that grow late."""
     B, n, D, P = 30, 2, 64, 700
