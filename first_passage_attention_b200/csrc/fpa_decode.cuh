@@ -341,8 +341,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
           l += w * p.part_ml[(pre + c) * 2 + 1];
           o += w * p.part_o[(pre + c) * D + d];
         }
-      // Rows before the sequence's first token see nothing.
-      out[row * p.so.t + d * p.so.d] = from_f32<O>(row < job.lead ? 0.f : o / l);
+      // Rows before the sequence's first token see nothing, nor does a row whose keys all lie in pages outside the pool.
+      out[row * p.so.t + d * p.so.d] = from_f32<O>(row < job.lead || l == 0.f ? 0.f : o / l);
     }
     if (S > 1) cluster_barrier();  // the other CTAs have read this one's shared memory
   }

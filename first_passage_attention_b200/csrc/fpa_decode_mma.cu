@@ -402,15 +402,17 @@ struct MmaCore {
     later.ids(c, job.table, job.t1 * kKeys, history > 0 ? job.end : 0);
     load_q<kPrefix>(p, job);
     int64_t base = -1;
-    auto fetch_block = [&](int i) {
-      const int lim = base < 0 ? 0 : min(kKeys, job.end - next * kKeys);
+    // Keys of the blocks on their way, the earliest first: none of a block whose page lies outside the pool.
+    int lims[kStages - 1] = {};
+    auto fetch_block = [&](int i, int& lim) {
+      lim = base < 0 ? 0 : min(kKeys, job.end - next * kKeys);
       fetch(c, ring + (i % kStages) * kStage, base < 0 ? 0 : base, lim);
       --next;
     };
     auto fetch_next = [&](int i) {
       // Block i of the run into its stage; the place of the one after it, where that lies in another page, is looked
       // up meanwhile.
-      fetch_block(i);
+      fetch_block(i, lims[kStages - 2]);
       if (i + 1 < history) {
         if (((next + 1) * kKeys & ((1 << c.page_shift) - 1)) != 0 && base >= 0)
           base -= kKeys;
@@ -420,13 +422,13 @@ struct MmaCore {
     };
     if (history > 0) {
       base = slot_in(c, pid0, job.h, next * kKeys);
-      fetch_block(0);
+      fetch_block(0, lims[0]);
     }
     if (history > 0 || !job.last) copy_commit();  // else the newest tokens' place is not known yet
     if constexpr (kStages == 3) {
       if (history > 1) {
         base = slot_in(c, pid1, job.h, next * kKeys);
-        fetch_block(1);
+        fetch_block(1, lims[1 % (kStages - 1)]);
       }
       if (history > 1 || !job.last) copy_commit();
       if (history > 2) base = slot_in(c, pid2, job.h, next * kKeys);
@@ -471,6 +473,9 @@ struct MmaCore {
     for (int i = 0; i < total; ++i) {
       copy_wait<kStages - 2>();
       __syncwarp();
+      const int lim = lims[0];
+#pragma unroll
+      for (int j = 1; j < kStages - 1; ++j) lims[j - 1] = lims[j];
       if (i + kStages - 1 < history)
         fetch_next(i + kStages - 1);
       else if (job.last && i + kStages - 1 == history)
@@ -487,8 +492,7 @@ struct MmaCore {
         ref[nt] = make_float2(m[nt][0] == -kInf ? 0.f : -m[nt][0], m[nt][1] == -kInf ? 0.f : -m[nt][1]);
       const float2 sign2 = make_float2(sign, sign);
       if (i < history) {
-        const int tile = job.t1 - 1 - i;
-        const Field f = field_of(p, st, lane < kKeys && tile * kKeys + lane < job.end);
+        const Field f = field_of(p, st, lane < lim);
         float all;
         const float suf = fminf(suffix_min(f.phi, all), mid);
         mid = fminf(mid, all);

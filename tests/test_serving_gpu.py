@@ -512,6 +512,71 @@ def test_refusals():
     assert LaunchStats.kernels == 0
 
 
+# ------------------------------------------------------------------------- keys that are not there, or not finite ----
+
+FORMS = [(F16, None), (F16, I8), (F32, None), (F32, I8)]
+
+
+def expected_rows(q, k, v, phi, psi, beta, n, storage, gone):
+    """As `expected`, without the keys that `gone` [T] marks; rows that see no key at all are zeros."""
+    if storage == I8:
+        k, v = quantise(k)[2], quantise(v)[2]
+    q, k, v, phi, psi, beta = (x.double().cuda() for x in (q, k, v, phi, psi, beta))
+    gone = gone.cuda()
+    phi = torch.where(gone, torch.inf, phi)
+    T, out = k.shape[1], []
+    for t in range(T - n, T):
+        least = phi[:, 1:t + 1].flip(-1).cummin(-1).values.flip(-1)
+        z = (k[:, :t + 1] @ q[:, t, :, None])[..., 0] / q.shape[-1] ** 0.5
+        z[:, :t] += beta[:, None] * (least - psi[:, :t]).clamp(max=0)
+        z = torch.where(gone[:t + 1], -torch.inf, z)
+        o = (z.softmax(-1)[:, None] @ v[:, :t + 1])[:, 0]
+        out.append(torch.zeros_like(o) if bool(gone[:t + 1].all()) else o)
+    return torch.stack(out, 1).cpu()
+
+
+@pytest.mark.parametrize("dtype,storage", FORMS)
+@pytest.mark.parametrize("D,page,L,n,P", [(64, 32, 1000, 1, 0), (64, 64, 1000, 3, 0), (128, 64, 333, 16, 0), (256, 32, 200, 2, 0), (16, 128, 900, 5, 0),
+                                          (64, 32, 150, 5, 700), (128, 64, 150, 6, 700), (32, 32, 40, 3, 300), (64, 32, 33, 1, 150)])
+def test_keys_behind_bad_pages_are_skipped(dtype, storage, D, page, L, n, P):
+    """Table entries outside the pool: the result is that of the remaining keys, whatever the sequence is split into. A
+    row that sees none is zero."""
+    H, B = 2, 5
+    q, k, v, phi, psi = sequence(B, H, L, D, dtype, seed=D + n)
+    table, n_pages = tables([L] * B + [P], page, seed=L)
+    table, ptable = table[:-1], table[-1, :-(-P // page)].contiguous()
+    cache = FPACache(n_pages, H, D, page, dtype, storage)
+    poison(cache)
+    fill(cache, table, [L] * B, k, v, phi, psi)
+    pages, npre = -(-L // page), ptable.numel()
+    bad = [[pages // 2], [0, pages - 1], list(range(pages // 3, pages - 1)), [pages - 1], list(range(pages))]
+    kw, pre, pgone = {}, None, torch.zeros(0, dtype=torch.bool)
+    if P:
+        pre = [x[0] for x in sequence(1, H, P, D, dtype, 7)]
+        fill(cache, ptable[None], [P], *(x[None] for x in pre[1:]))
+        pgone = torch.zeros(P, dtype=torch.bool)
+        for i, x in ((npre // 2, -5), (npre - 1, n_pages)):
+            ptable[i] = x
+            pgone[i * page:(i + 1) * page] = True
+        kw = dict(prefix_table=ptable, prefix_len=P)
+    gone = torch.zeros(B, L, dtype=torch.bool)
+    for b, drop in enumerate(bad):
+        for i in drop:
+            table[b, i] = (-1, n_pages, -2 ** 31, 2 ** 31 - 1)[(b + i) % 4]
+            gone[b, i * page:(i + 1) * page] = True
+    beta = torch.tensor([0.8, 1.3])
+    got = first_passage_decode(q[:, :, L - n:].cuda(), cache, table, i32([L] * B), beta.cuda(), **kw)
+    with pytest.raises(ValueError, match="outside"):
+        cache.check()
+    for b in range(B):
+        seq = [x[b] for x in (q, k, v, phi, psi)]
+        if P:
+            seq = [torch.cat([x, y], 1) for x, y in zip(pre, seq)]
+        want = expected_rows(*seq, beta, n, storage, torch.cat([pgone, gone[b]]))
+        assert torch.isfinite(got[b]).all()
+        assert_close(got[b], want, seq[2].abs().max().item(), dtype, b)
+
+
 # ------------------------------------------------------------------------------------------------ verification ----
 
 def verify_oracle(p, q, draft, u, noise, lens=None):
