@@ -61,9 +61,15 @@ extern "C" FPA_API int fpa_decode(FpaDecodeArgs* a, void* stream) {
   if (!a->q || !a->o || !a->beta || !a->table || !a->lengths) return invalid("fpa_decode: null tensor pointer");
   if (a->prefix_len < 0 || (a->prefix_len > 0 && (!a->prefix_table || int64_t(a->prefix_pages) * c.page_size < a->prefix_len)))
     return invalid("fpa_decode: the prefix is longer than the pages of its table");
-  // A CTA takes at least eight rows where there are as many, so these keep the grids' y and z extents below 65536.
-  if (a->B > 65535 || c.H > 32767 || (a->prefix_len > 0 && int64_t(a->B) * a->n > 65535 * 8)) {
-    set_last_error("fpa_decode: B above 65535, H above 32767 or B * n above 524280 with a prefix is not supported");
+  // The grids' y and z extents stay below 65536: B, and the row groups of all heads, or of the batch behind a prefix. fp16
+  // queries go in groups of at least eight rows.
+  auto groups = [&](int64_t rows) {
+    const int group = c.dtype == FPA_DTYPE_F16 ? 8 : ffma_group(c.D, rows);
+    return (rows + group - 1) / group;
+  };
+  if (a->B > 65535 || c.H > 32767 || c.H * groups(a->n) > 65535 || (a->prefix_len > 0 && groups(int64_t(a->B) * a->n) > 65535)) {
+    set_last_error("fpa_decode: B above 65535, H above 32767 (16383 for float32 with D above 64 and n above 12) or, with a "
+                   "prefix, B * n above 524280 (262140 for float32 with D above 64) is not supported");
     return FPA_ERR_UNSUPPORTED;
   }
   DecodeParams p{};

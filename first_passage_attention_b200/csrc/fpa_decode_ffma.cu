@@ -342,25 +342,24 @@ struct FfmaCore {
   }
 };
 
-// Rows of a group: 1, 4, or, for D <= 64 and more than 4 rows, 8. Measured on 8 x 8 (sequence, head) pairs of 4096 tokens,
-// us for groups of 1 / 4 / 8: 8 rows, D = 32 int8 84 / 41 / 38, D = 64 147 / 88 / 87, D = 128 246 / 134 / 135; 2000 tokens at D =
-// 256 200 / 100 / 127 (the registers of 8 rows leave fewer CTAs); 2 rows, D = 32 29 / 25 / 37.
+template <int D, bool kInt8>
+cudaError_t launch_groups(const DecodeParams& p, bool prefix, cudaStream_t s, int& launches) {
+  const int group = ffma_group(D, prefix ? p.B * p.n : p.n);
+  if (group == 1) return launch_decode_core<FfmaCore<D, kInt8, 1>>(p, prefix, s, launches);
+  if constexpr (D <= 64) {
+    if (group == 8) return launch_decode_core<FfmaCore<D, kInt8, 8>>(p, prefix, s, launches);
+  }
+  return launch_decode_core<FfmaCore<D, kInt8, 4>>(p, prefix, s, launches);
+}
+
 template <bool kInt8>
 cudaError_t launch_for(const DecodeParams& p, bool prefix, cudaStream_t s, int& launches) {
-  const int rows = prefix ? p.B * p.n : p.n;
   switch (p.c.D) {
-#define FPA_CASE(D)                                                                                \
-  case D:                                                                                          \
-    return rows == 1 ? launch_decode_core<FfmaCore<D, kInt8, 1>>(p, prefix, s, launches)                     \
-           : rows < 5 || D > 64                                                                    \
-               ? launch_decode_core<FfmaCore<D, kInt8, 4>>(p, prefix, s, launches)                           \
-               : launch_decode_core<FfmaCore<D, kInt8, D <= 64 ? 8 : 4>>(p, prefix, s, launches);
-    FPA_CASE(16)
-    FPA_CASE(32)
-    FPA_CASE(64)
-    FPA_CASE(128)
-    FPA_CASE(256)
-#undef FPA_CASE
+    case 16: return launch_groups<16, kInt8>(p, prefix, s, launches);
+    case 32: return launch_groups<32, kInt8>(p, prefix, s, launches);
+    case 64: return launch_groups<64, kInt8>(p, prefix, s, launches);
+    case 128: return launch_groups<128, kInt8>(p, prefix, s, launches);
+    case 256: return launch_groups<256, kInt8>(p, prefix, s, launches);
     default:
       return cudaErrorInvalidValue;
   }

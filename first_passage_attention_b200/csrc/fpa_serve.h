@@ -64,7 +64,11 @@ struct DecodeParams {
   bool followed, follows;
 };
 
-// Rows are handled by one CTA in groups of 8 or 16 (tensor cores) or 1, 4 or 8 (FFMA).
+// Rows are handled by one CTA in groups of 8 or 16 (tensor cores) or 1, 4 or 8 (FFMA). For FFMA, 8 for D <= 64 and more than 4
+// rows. Measured on 8 x 8 (sequence, head) pairs of 4096 tokens, us for groups of 1 / 4 / 8: 8 rows, D = 32 int8 84 / 41 / 38,
+// D = 64 147 / 88 / 87, D = 128 246 / 134 / 135; 2000 tokens at D = 256 200 / 100 / 127 (the registers of 8 rows leave fewer
+// CTAs); 2 rows, D = 32 29 / 25 / 37.
+inline int ffma_group(int D, int64_t rows) { return rows == 1 ? 1 : rows < 5 || D > 64 ? 4 : 8; }
 cudaError_t launch_decode_mma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s, int& launches);
 cudaError_t launch_decode_ffma(const DecodeParams& p, bool int8, bool prefix, cudaStream_t s, int& launches);
 // The prefix on tcgen05: fp16 queries, D = 64 or 128. p.chunks: CTAs that share a row tile's prefix.

@@ -68,6 +68,31 @@ def test_argument_errors_come_before_any_cuda_call():
         assert got == rc and message in lib.fpa_last_error(), (message, got, lib.fpa_last_error())
 
 
+def test_row_groups_fit_the_grid():
+    """float32 rows with D = 128 and 256 go in groups of four: their grids are full at half of the rows and heads."""
+    lib = _lib.load()
+    dec = dict(max_pages=1, q=4096, o=4096, beta=4096, table=4096, lengths=4096)
+    pre = dict(prefix_len=64, prefix_pages=1, prefix_table=4096)  # without a workspace: what passes the check ends there
+    f32 = dict(dtype=_lib.DTYPE_F32, storage=_lib.STORE_F32)
+    for cache, args, rc in [
+            (dict(f32, D=128, H=16384), dict(B=1, n=13, **pre), _lib.ERR_UNSUPPORTED),
+            (dict(f32, D=256, H=32767), dict(B=1, n=16, **pre), _lib.ERR_UNSUPPORTED),
+            (dict(f32, D=128, H=16383), dict(B=1, n=16, **pre), _lib.ERR_WORKSPACE),
+            (dict(f32, D=128, H=21845), dict(B=1, n=12, **pre), _lib.ERR_WORKSPACE),
+            (dict(f32, D=64, H=32767), dict(B=1, n=16, **pre), _lib.ERR_WORKSPACE),
+            (dict(D=128, H=32767), dict(B=1, n=16, **pre), _lib.ERR_WORKSPACE),
+            (dict(f32, D=128, H=2), dict(B=20165, n=13, **pre), _lib.ERR_UNSUPPORTED),
+            (dict(f32, D=256, H=2), dict(B=65535, n=4, **pre), _lib.ERR_WORKSPACE),
+            (dict(f32, D=256, H=2), dict(B=65535, n=5, **pre), _lib.ERR_UNSUPPORTED),
+            (dict(f32, D=64, H=2), dict(B=65535, n=8, **pre), _lib.ERR_WORKSPACE),
+            (dict(f32, D=64, H=2), dict(B=65535, n=9, **pre), _lib.ERR_UNSUPPORTED),
+            (dict(D=256, H=2), dict(B=65535, n=8, **pre), _lib.ERR_WORKSPACE),
+            (dict(D=128, H=2), dict(B=65535, n=16, **pre), _lib.ERR_UNSUPPORTED)]:
+        c = _cache(**cache)
+        got = lib.fpa_decode(ctypes.byref(_lib.FpaDecodeArgs(cache=ctypes.addressof(c), **dec, **args)), None)
+        assert got == rc, (cache, args, got, lib.fpa_last_error())
+
+
 def test_workspace_grows_with_the_rows_of_a_prefix_only():
     lib = _lib.load()
     c = _cache()
