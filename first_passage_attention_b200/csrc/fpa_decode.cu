@@ -45,7 +45,7 @@ size_t workspace_bytes(const FpaCache& c, int B, int n, int prefix_len, size_t* 
 using namespace fpa;
 
 extern "C" FPA_API size_t fpa_decode_workspace_bytes(const FpaCache* cache, int B, int n, int prefix_len) {
-  if (check_cache(cache) || B <= 0 || n <= 0 || n > kMaxNew) return 0;
+  if (check_cache(cache) || B <= 0 || n <= 0 || n > kMaxNew || prefix_len > kMaxPositions) return 0;
   size_t ml, o;
   return workspace_bytes(*cache, B, n, prefix_len, &ml, &o);
 }
@@ -61,6 +61,10 @@ extern "C" FPA_API int fpa_decode(FpaDecodeArgs* a, void* stream) {
   if (!a->q || !a->o || !a->beta || !a->table || !a->lengths) return invalid("fpa_decode: null tensor pointer");
   if (a->prefix_len < 0 || (a->prefix_len > 0 && (!a->prefix_table || int64_t(a->prefix_pages) * c.page_size < a->prefix_len)))
     return invalid("fpa_decode: the prefix is longer than the pages of its table");
+  if (a->prefix_len > kMaxPositions) {
+    set_last_error("fpa_decode: prefixes above 2147483392 tokens are not supported");
+    return FPA_ERR_UNSUPPORTED;
+  }
   // The grids' y and z extents stay below 65536: B, and the row groups of all heads, or of the batch behind a prefix. fp16
   // queries go in groups of at least eight rows.
   auto groups = [&](int64_t rows) {

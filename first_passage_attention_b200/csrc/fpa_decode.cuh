@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Core::kMinBlocks) decode_kerne
   } else {
     job.h = blockIdx.y / p.groups;
     job.r0 = (blockIdx.y - job.h * p.groups) * NQ;
-    const int cap = int(min(int64_t(p.max_pages) << p.c.page_shift, int64_t(INT32_MAX)));
+    const int cap = int(min(int64_t(p.max_pages) << p.c.page_shift, int64_t(kMaxPositions)));
     job.b = kSorted ? by_length(p.lengths, p.B, p.first + blockIdx.z, cap) : p.first + blockIdx.z;
     job.table = p.table + job.b * p.table_stride;
     int L = p.lengths[job.b];

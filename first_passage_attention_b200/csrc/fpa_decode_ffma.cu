@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(128) row_min_kernel(const __grid_constant__ De
   if (i >= p.B * p.c.H) return;
   const int b = i / p.c.H, h = i - b * p.c.H;
   const int32_t* table = p.table + b * p.table_stride;
-  const int cap = int(min(int64_t(p.max_pages) << p.c.page_shift, int64_t(INT32_MAX)));
+  const int cap = int(min(int64_t(p.max_pages) << p.c.page_shift, int64_t(kMaxPositions)));
   const int L = min(max(p.lengths[b], 0), cap), Lb = max(L - p.n, 0), nn = L - Lb, lead = p.n - nn;
   const int pid = lane < nn ? table[(Lb + lane) >> p.c.page_shift] : -1;
   LaterMin own;

@@ -6,6 +6,8 @@
 namespace fpa {
 
 constexpr int kMaxNew = 16;  // newest tokens of one decode call
+// Positions of a sequence, or of a prefix, that decode takes: rounding one up to a page or a tile stays within 32 bits.
+constexpr int kMaxPositions = INT32_MAX - 255;
 
 // Sites that the cache's status word names next to FPA_ERR_INVALID_ARGUMENT.
 enum ServeSite { kSiteAppend = 1, kSiteRead = 2, kSiteDecode = 3 };

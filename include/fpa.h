@@ -173,7 +173,7 @@ typedef struct FpaReadArgs {
 
 /* Attention of the newest n tokens of each sequence (1 <= n <= 16), which are in the cache already: lengths[b] counts
  * them, and row r of sequence b stands at its position lengths[b] - n + r. Rows at negative positions come out as
- * zeros (a sequence of length 0 is an idle slot). With a prefix (prefix_len > 0), the prefix's tokens, which lie in
+ * zeros (a sequence of length 0 is an idle slot). Lengths end at the table's row, and at 2^31 - 256. With a prefix (prefix_len > 0), the prefix's tokens, which lie in
  * the pages of prefix_table, come before the first token of every sequence; lengths do not count them. */
 typedef struct FpaDecodeArgs {
   const FpaCache* cache;

@@ -93,6 +93,16 @@ def test_row_groups_fit_the_grid():
         assert got == rc, (cache, args, got, lib.fpa_last_error())
 
 
+def test_prefixes_end_where_positions_round_up_within_32_bits():
+    lib = _lib.load()
+    c = _cache()
+    dec = dict(cache=ctypes.addressof(c), B=1, n=1, max_pages=1, q=4096, o=4096, beta=4096, table=4096, lengths=4096,
+               prefix_table=4096, prefix_pages=2 ** 25)
+    for length, rc in ((2 ** 31 - 256, _lib.ERR_WORKSPACE), (2 ** 31 - 255, _lib.ERR_UNSUPPORTED), (2 ** 31 - 1, _lib.ERR_UNSUPPORTED)):
+        assert lib.fpa_decode(ctypes.byref(_lib.FpaDecodeArgs(prefix_len=length, **dec)), None) == rc, length
+        assert (lib.fpa_decode_workspace_bytes(ctypes.byref(c), 1, 1, length) > 0) == (rc == _lib.ERR_WORKSPACE)
+
+
 def test_workspace_grows_with_the_rows_of_a_prefix_only():
     lib = _lib.load()
     c = _cache()

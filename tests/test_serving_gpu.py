@@ -577,6 +577,23 @@ def test_keys_behind_bad_pages_are_skipped(dtype, storage, D, page, L, n, P):
         assert_close(got[b], want, seq[2].abs().max().item(), dtype, b)
 
 
+def test_lengths_at_the_end_of_32_bits():
+    """A table of 2^31 positions, all in one page: lengths end where rounding up to a page stays within 32 bits."""
+    H, D, page = 1, 16, 256
+    q, k, v, phi, psi = sequence(1, H, page, D, F16, seed=15)
+    cache = FPACache(1, H, D, page, F16)
+    table = torch.zeros(1, 2 ** 31 // page, dtype=torch.int32, device="cuda")
+    cache.append(k.cuda(), v.cuda(), phi.cuda(), psi.cuda(), table, i32([0]))
+    for length, ok in ((2 ** 31 - 256, True), (2 ** 31 - 1, False)):
+        got = first_passage_decode(q[:, :, :1].cuda(), cache, table, i32([length]), torch.ones(H, device="cuda"))
+        assert torch.isfinite(got).all()
+        if ok:
+            cache.check()
+        else:
+            with pytest.raises(ValueError, match="outside"):
+                cache.check()
+
+
 # ------------------------------------------------------------------------------------------------ verification ----
 
 def verify_oracle(p, q, draft, u, noise, lens=None):
