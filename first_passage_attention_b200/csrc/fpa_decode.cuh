@@ -41,6 +41,14 @@ __device__ __forceinline__ int64_t slot_of(const CacheView& c, const int32_t* ta
   return slot_in(c, table[pos >> c.page_shift], h, pos);
 }
 
+// phi of a position whose page's id is given; 0 where that lies outside the pool or phi is not finite. What M and psi are
+// counted from where they are scaled apart from each other: the walk may stand anywhere, the bias is made of differences.
+__device__ __forceinline__ float level_at(const CacheView& c, int pid, int h, int pos) {
+  if (unsigned(pid) >= unsigned(c.n_pages)) return 0.f;
+  const float x = c.phi[((int64_t(pid) * c.H + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1))];
+  return fabsf(x) < kInf ? x : 0.f;
+}
+
 // The warp's minimum of phi over the positions [from, to) of a sequence: whole pages through phi_min, the rest from
 // phi itself. In three steps, so that the table's entries, and then the values, of this and of the caller's other
 // look-ups travel together.

@@ -360,8 +360,10 @@ struct MmaCore {
   }
 
   // This lane's key of the stage: its field and scales. With b' = beta log2(e), the bias plus lv of a row is b' min(a_s,
-  // M - psi_s) + lv, which times the sign of b' is min(a, low + e) for a = |b'| a_s + sign lv, e = -|b'| psi_s + sign lv
-  // and the row's low = |b'| M; sign f is the product's factor. No such key: a = e = -sign inf.
+  // M - psi_s) + lv, which times the sign of b' is min(a, low + e) for a = |b'| a_s + sign lv, e = -|b'| (psi_s - level) +
+  // sign lv and the row's low = |b'| (M - level); sign f is the product's factor. No such key: a = e = -sign inf. The level
+  // is phi of the first new token (of the prefix's last token), which M is near to, and psi_s too wherever the bias is
+  // small: what is rounded here is then of the bias's own size, however far from zero the walk stands.
   struct Field {
     float phi, psi, f, lv, rv;
   };
@@ -397,6 +399,7 @@ struct MmaCore {
     const int pid0 = history > 0 ? job.table[(next * kKeys) >> c.page_shift] : -1;
     const int pid1 = history > 1 ? job.table[((next - 1) * kKeys) >> c.page_shift] : -1;
     const int pid2 = kStages == 3 && history > 2 ? job.table[((next - 2) * kKeys) >> c.page_shift] : -1;
+    const int pid_level = kPrefix ? job.table[(job.end - 1) >> c.page_shift] : -1;
     const int pid_new = !kPrefix && lane < job.n_new ? job.table[(job.end + lane) >> c.page_shift] : -1;
     LaterMin later;
     later.ids(c, job.table, job.t1 * kKeys, history > 0 ? job.end : 0);
@@ -438,6 +441,13 @@ struct MmaCore {
     NewTokens nw{kInf, 0.f, kInf, -1, 0};
     if constexpr (!kPrefix) nw = load_new(c, pid_new, job.h, job.end, job.n_new);
     later.values(c, job.h);
+    float level;
+    if constexpr (kPrefix) {
+      level = level_at(c, pid_level, job.h, job.end - 1);
+    } else {
+      level = __shfl_sync(0xffffffffu, nw.phi, 0);
+      if (!(fabsf(level) < kInf)) level = 0.f;  // no new token, or a page outside the pool
+    }
     sum_q();
     nw.low = prefix_min(nw.phi);
     sign = job.bias < 0.f ? -1.f : 1.f;
@@ -465,7 +475,7 @@ struct MmaCore {
           if (i < 0 || i >= job.n_new) x = kInf;
         }
         // strength 0: the bias is 0 whatever the minimum is (not 0 times infinity).
-        low[nt][q] = strength == 0.f ? 0.f : strength * x;
+        low[nt][q] = strength == 0.f ? 0.f : strength * (x - level);
 #pragma unroll
         for (int j = 0; j < MT; ++j) o[j][nt][q] = o[j][nt][q + 2] = 0.f;
       }
@@ -497,7 +507,7 @@ struct MmaCore {
         const float suf = fminf(suffix_min(f.phi, all), mid);
         mid = fminf(mid, all);
         if (lane < kKeys)
-          par[lane] = make_float4(fmaf(-strength, f.psi, sign * f.lv), fmaf(strength, fminf(suf - f.psi, 0.f), sign * f.lv),
+          par[lane] = make_float4(fmaf(-strength, f.psi - level, sign * f.lv), fmaf(strength, fminf(suf - f.psi, 0.f), sign * f.lv),
                                   sign * f.f, f.rv);
         __syncwarp();
 #pragma unroll

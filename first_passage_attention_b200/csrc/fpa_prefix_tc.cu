@@ -124,6 +124,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   const int each = tiles / S, more = tiles - each * S;
   const int t0 = int(blockIdx.x) * each + min(int(blockIdx.x), more);
   const int nt = each + (int(blockIdx.x) < more ? 1 : 0), t1 = t0 + nt;
+  auto prefix_level = [&]() {
+    return level_at(c, p.prefix_table[(p.prefix_len - 1) >> c.page_shift], h, p.prefix_len - 1);
+  };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::SLOTS; ++i) mbar_init(full + i, kLoaders);
@@ -342,8 +345,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     } else if (warp < kWarpField + 2) {
       // ----------------------------------------------------------------------- the keys' field and scales ----
       // Per key, with b' = beta log2(e) and lv = log2 of V's scale (0 in fp16): the bias plus lv of a row is the smaller
-      // (b' < 0: the larger) of a = b' min(SUF - psi, 0) + lv and b' M + e, e = -b' psi + lv; -inf where there is no key.
-      const float bias = p.beta[h] * kLog2e;
+      // (b' < 0: the larger) of a = b' min(SUF - psi, 0) + lv and b' (M - level) + e, e = -b' (psi - level) + lv; -inf where
+      // there is no key. The level is phi of the prefix's last token (see fpa_decode_mma.cu).
+      const float bias = p.beta[h] * kLog2e, level = prefix_level();
       // Two warps take alternate tiles; each also reads the phi of the tiles between its own, for the minimum.
       const int first = warp - kWarpField;
       float mid = t1 * kTile < p.prefix_len ? later_min(c, p.prefix_table, h, t1 * kTile, p.prefix_len) : kInf;
@@ -422,7 +426,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
             rv[j] = ok ? rcp_approx_f(v) : 0.f;
           }
           a[j] = ok ? fmaf(bias, fminf(suf - ps[j], 0.f), lv) : -kInf;
-          e[j] = ok ? fmaf(-bias, ps[j], lv) : -kInf;
+          e[j] = ok ? fmaf(-bias, ps[j] - level, lv) : -kInf;
           suf = fminf(suf, f[j]);
         }
         float* out = reinterpret_cast<float*>(smem + C::OFF_PAR + st * C::PARB);
@@ -483,11 +487,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     const bool busy = lr - lane < rows;       // some row of this warp exists (RP is a multiple of 32)
     const uint32_t tl = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t tO = tl + C::COL_O + g * D;
+    const float level = prefix_level();
     pdl_wait();  // row_min
     pdl_launch_dependents();
     const float low = lr < rows ? p.row_min[int64_t(h) * R + r0 + lr] : kInf;
     const float bias = p.beta[h] * kLog2e;
-    const float2 low2 = make_float2(bias * low, bias * low), sc2 = make_float2(p.scale2, p.scale2);
+    const float2 low2 = make_float2(bias * (low - level), bias * (low - level)), sc2 = make_float2(p.scale2, p.scale2);
     float m = -kInf;
     float2 l2 = make_float2(0.f, 0.f);
     bool ok = true;

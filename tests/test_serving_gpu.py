@@ -577,6 +577,37 @@ def test_keys_behind_bad_pages_are_skipped(dtype, storage, D, page, L, n, P):
         assert_close(got[b], want, seq[2].abs().max().item(), dtype, b)
 
 
+@pytest.mark.parametrize("dtype,storage", FORMS)
+@pytest.mark.parametrize("D,n,P", [(64, 2, 0), (128, 5, 0), (256, 3, 0), (32, 3, 400), (256, 2, 300), (64, 5, 700), (128, 3, 700)])
+@pytest.mark.parametrize("offset,slope,sign", [(1e6, 0.0, 1), (-1e6, 0.0, -1), (0.0, -4.0, 1), (3e5, -1.0, 1)])
+def test_a_walk_far_from_zero(dtype, storage, D, n, P, offset, slope, sign):
+    """The bias depends on differences of the field only: a walk that starts far from zero or falls steadily costs no
+    accuracy (an offset of 1e6 is held in steps of 1/16, a logit off by such a step would show at 6e-2)."""
+    H, lens = 2, [700, 33, 64, 500, 150, 9]
+    B, T = len(lens), max(lens)
+    drift = offset + slope * torch.arange(P + T, dtype=torch.float32)
+    q, k, v, phi, psi = sequence(B, H, T, D, dtype, seed=D + n)
+    phi, psi = phi + drift[P:], psi + drift[P:]
+    table, n_pages = tables(lens + [P], 64, seed=n)
+    table, ptable = table[:-1], table[-1, :-(-P // 64)].contiguous()
+    cache = FPACache(n_pages, H, D, 64, dtype, storage)
+    fill(cache, table, lens, k, v, phi, psi)
+    kw, pre = {}, None
+    if P:
+        pre = [x[0] for x in sequence(1, H, P, D, dtype, 5)]
+        pre[3], pre[4] = pre[3] + drift[:P], pre[4] + drift[:P]
+        fill(cache, ptable[None], [P], *(x[None] for x in pre[1:]))
+        kw = dict(prefix_table=ptable, prefix_len=P)
+    beta = sign * torch.tensor([0.8, 1.3])
+    newest = torch.stack([q[b, :, L - n:L] for b, L in enumerate(lens)]).cuda()
+    got = first_passage_decode(newest, cache, table, i32(lens), beta.cuda(), **kw)
+    for b, L in enumerate(lens):
+        seq = [x[b, :, :L] for x in (q, k, v, phi, psi)]
+        if P:
+            seq = [torch.cat([x, y], 1) for x, y in zip(pre, seq)]
+        assert_close(got[b], expected(*seq, beta, n, storage), seq[2].abs().max().item(), dtype, (b, L))
+
+
 def test_lengths_at_the_end_of_32_bits():
     """A table of 2^31 positions, all in one page: lengths end where rounding up to a page stays within 32 bits."""
     H, D, page = 1, 16, 256
