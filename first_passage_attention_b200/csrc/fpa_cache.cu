@@ -38,7 +38,8 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8], float top) {
     w[j] = __float_as_uint(r.x);
     w[j + 1] = __float_as_uint(r.y);
   }
-  if (!(off < 0.5f - 0x1p-14f) || !(top < 0x1p100f)) {  // near a half, or the reciprocal leaves float32's normal range
+  // Near a half, or the reciprocal leaves float32's normal range, or NaN (codes 0).
+  if (!(off < 0.5f - 0x1p-14f) || !(top < 0x1p100f)) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       w[j] = min(max(__float2int_rn(__fdiv_rn(__fmul_rn(x[j], 127.f), top)), -127), 127) + 128;
@@ -196,13 +197,14 @@ __global__ void __launch_bounds__(kMaxThreads, 4) append_kernel(const __grid_con
       if constexpr (kInt8) {
         float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[a][j]));
+        for (int j = 0; j < 8; ++j) m = fmax_nan(m, fabsf(x[a][j]));
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1)
-          if (o < lanes) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          if (o < lanes) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
         // Scales stay at or above 2^-90, so that their inverses sum up in float32 (see fpa_decode_mma.cu); a row of
-        // zeros takes that smallest scale, so that it does not outweigh small rows there.
-        top[a] = fmaxf(m, 127.f * 0x1p-90f);
+        // zeros takes that smallest scale, so that it does not outweigh small rows there. A row with a NaN or an infinity
+        // has no codes: its scale is NaN.
+        top[a] = m < kInf ? fmaxf(m, 127.f * 0x1p-90f) : __int_as_float(0x7fffffff);
         const uint2 w = encode8(x[a], top[a]);
         if (ok) *reinterpret_cast<uint2*>(dst + a * dst_step) = w;
       } else if (ok) {

@@ -36,6 +36,13 @@ __device__ __forceinline__ float rcp_approx_f(float x) {
   return y;
 }
 
+// Maximum that is NaN where an operand is (fmaxf drops it).
+__device__ __forceinline__ float fmax_nan(float x, float y) {
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
 __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -293,10 +293,10 @@ struct FfmaCore {
       __syncwarp();
       float f = p.scale2, lv = ok ? 0.f : -kInf, rv = 1.f;
       if (kInt8 && ok) {
-        const float v = fmaxf(f_vs, 0x1p-90f);
+        const float v = fmax_nan(f_vs, 0x1p-90f);
         f *= f_ks;
         lv = lg2(v);
-        rv = 1.f / v;
+        rv = v != v ? 1.f : 1.f / v;  // NaN reaches the rows that see the key through lv, and no other
       }
       if (!fresh) {
         float all;

@@ -380,10 +380,11 @@ struct MmaCore {
       f.f = p.scale2;
       f.lv = 0.f;
       if constexpr (kInt8) {
-        const float v = fmaxf(word(3), 0x1p-90f);
+        const float v = fmax_nan(word(3), 0x1p-90f);
         f.f *= word(2) * 0x1p24f;
         f.lv = lg2(v);
         f.rv = rcp_approx_f(v);
+        if (v != v) f.rv = 1.f;  // NaN reaches the rows that see the key through lv, and no other
       }
     }
     return f;

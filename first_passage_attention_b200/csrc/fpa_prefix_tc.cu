@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
           const bool ok = j < left;
           float lv = 0.f;
           if constexpr (kInt8) {
-            const float v = fmaxf(vs[j], 0x1p-90f);
+            const float v = fmax_nan(vs[j], 0x1p-90f);
             fac[j] = ks[j] * p.scale2;
             lv = lg2(v);
             rv[j] = ok ? rcp_approx_f(v) : 0.f;

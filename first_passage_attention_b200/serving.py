@@ -71,7 +71,7 @@ class FPACache:
 
     dtype: of k, v, q and o (float16 or float32). storage: None (as dtype) or torch.int8: scale = max|x| / 127 for each
     token and head (at least 2^-90), code = round(127 x / max|x|), the value is code * scale; the pool holds code + 128 as
-    uint8."""
+    uint8. A row with a NaN or an infinity gets the scale NaN: it reads back as NaN, and so does what attends to it."""
 
     def __init__(self, n_pages, n_heads, head_dim, page_size=64, dtype=torch.float16, storage=None, device="cuda"):
         if dtype not in (torch.float16, torch.float32):

@@ -146,7 +146,8 @@ typedef struct FpaCache {
 
 /* Appends counts[b] tokens (all n if counts is null) to each sequence at its positions start[b], start[b] + 1, ...
  * Later positions of the sequence are no longer part of it. int8: scale = max|x| / 127 (at least 2^-90), code =
- * rint(127 x / max|x|), the value is code * scale. phi_min of the touched pages is brought up to date. */
+ * rint(127 x / max|x|), the value is code * scale; a row with a NaN or an infinity gets the scale NaN and codes 0.
+ * phi_min of the touched pages is brought up to date. */
 typedef struct FpaAppendArgs {
   const FpaCache* cache;
   int32_t B, n;

@@ -608,6 +608,51 @@ def test_a_walk_far_from_zero(dtype, storage, D, n, P, offset, slope, sign):
         assert_close(got[b], expected(*seq, beta, n, storage), seq[2].abs().max().item(), dtype, (b, L))
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D,P", [(64, 0), (128, 0), (16, 0), (64, 300), (128, 300), (256, 200)])
+def test_int8_rows_that_are_not_finite(dtype, D, P):
+    """A row of keys or values with a NaN or an infinity has no codes: it reads back as NaN, and what attends to it is NaN.
+    Other rows, sequences and heads are as they were."""
+    H, L, n, page = 2, 100, 3, 32
+    q, k, v, phi, psi = sequence(6, H, L, D, dtype, seed=D)
+    table, n_pages = tables([L] * 6 + [P], page)
+    table, ptable = table[:-1], table[-1, :-(-P // page)].contiguous()
+    cache = FPACache(n_pages, H, D, page, dtype, I8)
+    kw, pre = {}, None
+    if P:
+        pre = [x[0] for x in sequence(1, H, P, D, dtype, 3)]
+        fill(cache, ptable[None], [P], *(x[None] for x in pre[1:]))
+        kw = dict(prefix_table=ptable, prefix_len=P)
+    nan, inf = float("nan"), float("inf")
+    bad = {0: (k, 40, nan), 1: (v, 41, nan), 2: (k, 42, inf), 3: (v, 43, -inf)}
+    for b, (x, s, value) in bad.items():
+        x[b, 0, s, (7 * b) % D] = value
+    fill(cache, table, [L] * 6, k, v, phi, psi)
+    back = cache.read(table, None, L)
+    for b, (x, s, _) in bad.items():
+        r = back[0 if x is k else 1][b].cpu()
+        assert torch.isnan(r[0, s]).all()
+        keep = torch.ones(H, L, dtype=torch.bool)
+        keep[0, s] = False
+        assert torch.equal(r[keep], quantise(x[b][keep])[2].to(dtype))
+    beta = torch.tensor([0.0, 1.0])  # head 0 without the bias: every key counts
+    got = first_passage_decode(q[:, :, L - n:].cuda(), cache, table, i32([L] * 6), beta.cuda(), **kw)
+    for b in range(6):
+        seq = [x[b] for x in (q, k, v, phi, psi)]
+        if P:
+            seq = [torch.cat([x, y], 1) for x, y in zip(pre, seq)]
+        heads = slice(1, 2) if b in bad else slice(0, 2)
+        if b in bad:
+            assert torch.isnan(got[b, 0]).all(), b
+        want = expected(*(x[heads] for x in seq), beta[heads], n, I8)
+        assert_close(got[b, heads], want, max(x[heads].abs().max().item() for x in seq[2:3]), dtype, b)
+    if P:  # a value of the prefix that is not finite reaches every row
+        pre[2][0, 77, 1] = nan
+        fill(cache, ptable[None], [P], *(x[None] for x in pre[1:]))
+        got = first_passage_decode(q[:, :, L - n:].cuda(), cache, table, i32([L] * 6), beta.cuda(), **kw)
+        assert torch.isnan(got[:, 0]).all() and torch.isfinite(got[:, 1]).all()
+
+
 def test_lengths_at_the_end_of_32_bits():
     """A table of 2^31 positions, all in one page: lengths end where rounding up to a page stays within 32 bits."""
     H, D, page = 1, 16, 256
