@@ -40,9 +40,11 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8], float top) {
   }
   // Near a half, or the reciprocal leaves float32's normal range, or NaN (codes 0).
   if (!(off < 0.5f - 0x1p-14f) || !(top < 0x1p100f)) {
+    // 127 x would leave float32 for the largest rows: those are scaled down, which is exact where it matters.
+    const float down = top < 0x1p100f ? 1.f : 0x1p-20f;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      w[j] = min(max(__float2int_rn(__fdiv_rn(__fmul_rn(x[j], 127.f), top)), -127), 127) + 128;
+      w[j] = min(max(__float2int_rn(__fdiv_rn(__fmul_rn(x[j] * down, 127.f), top * down)), -127), 127) + 128;
   }
   auto four = [&](int j) {
     return __byte_perm(__byte_perm(w[j], w[j + 1], 0x0040), __byte_perm(w[j + 2], w[j + 3], 0x0040), 0x5410);

@@ -653,6 +653,25 @@ def test_int8_rows_that_are_not_finite(dtype, D, P):
         assert torch.isnan(got[:, 0]).all() and torch.isfinite(got[:, 1]).all()
 
 
+def test_int8_rows_near_the_end_of_float32():
+    """127 x overflows from 2.7e36 on; the codes do not."""
+    H, D, n = 2, 32, 6
+    _, k, v, phi, psi = sequence(1, H, n, D, F32, seed=4)
+    for i, top in enumerate((3.0e38, 1e37, 3e36, 2e36, 1.3e30, 1.2e30)):
+        k[0, :, i] = k[0, :, i] / k[0, :, i].abs().amax(-1, keepdim=True) * top
+        v[0, :, i] = v[0, :, i] / v[0, :, i].abs().amax(-1, keepdim=True) * top
+    table, n_pages = tables([n], 32)
+    cache = FPACache(n_pages, H, D, 32, F32, I8)
+    fill(cache, table, [n], k, v, phi, psi)
+    for x, pool, scales in ((k, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
+        top = x[0].double().abs().amax(-1, keepdim=True)
+        exact = x[0].double() * 127 / top
+        codes = pool[table[0, 0], :, :n].cpu().double() - 128
+        # A code next to the exact quotient; the nearest one unless the quotient is within float32 rounding of a half.
+        assert ((codes - exact).abs() <= 0.5 + 1e-4).all()
+        assert (scales[table[0, 0], :, :n].cpu().double() * 127 / top[..., 0] - 1).abs().max().item() <= 2.0 ** -22
+
+
 def test_lengths_at_the_end_of_32_bits():
     """A table of 2^31 positions, all in one page: lengths end where rounding up to a page stays within 32 bits."""
     H, D, page = 1, 16, 256
