@@ -155,8 +155,11 @@ struct FfmaCore {
     }
   }
 
-  // O += P V of the eight keys in stage i, columns first .. first + 7 of P.
+  // O += P V of the eight keys in stage i, columns first .. first + 7 of P. kMasked: some rows do not see all of these keys;
+  // what they do not see stays out of their sums even where it is not finite.
+  template <bool kMasked>
   __device__ __forceinline__ void values(int i, int first) {
+    auto add = [](float e, float v, float x) { return kMasked && e == 0.f ? x : fmaf(e, v, x); };
     const char* rows = ring_ptr + (i % kStages) * kStage;
     if constexpr (KG > 1) {
 #pragma unroll
@@ -165,7 +168,7 @@ struct FfmaCore {
         float v[CPL];
         load_v(rows + k * kPitch, v);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) o[r][0] = fmaf(ss[r * 32 + first + k], v[0], o[r][0]);
+        for (int r = 0; r < NR; ++r) o[r][0] = add(ss[r * 32 + first + k], v[0], o[r][0]);
       }
     } else {
 #pragma unroll
@@ -179,10 +182,10 @@ struct FfmaCore {
 #pragma unroll
           for (int j = 0; j < CPL; ++j) {
             float x = o[r][j];
-            x = fmaf(e.x, v[0][j], x);
-            x = fmaf(e.y, v[1][j], x);
-            x = fmaf(e.z, v[2][j], x);
-            o[r][j] = fmaf(e.w, v[3][j], x);
+            x = add(e.x, v[0][j], x);
+            x = add(e.y, v[1][j], x);
+            x = add(e.z, v[2][j], x);
+            o[r][j] = add(e.w, v[3][j], x);
           }
         }
       }
@@ -314,7 +317,10 @@ struct FfmaCore {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         next(8 * k + 4 + j);
-        values(8 * k + 4 + j, j * 8);
+        if (fresh)
+          values<true>(8 * k + 4 + j, j * 8);
+        else
+          values<false>(8 * k + 4 + j, j * 8);
       }
     }
     copy_wait<0>();

@@ -390,6 +390,60 @@ struct MmaCore {
     return f;
   }
 
+  // The newest tokens' values in fp16 may hold infinities and NaN, which a product with a weight of zero would bring to the
+  // rows that do not see the token. Such elements count as zeros in the tile's products (true if there are any) ...
+  __device__ __forceinline__ bool clear_wild(uint32_t st) {
+    const uint32_t v = st + kArray + lane * 16;
+    auto load = [](uint32_t at) {
+      uint4 w;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
+      return w;
+    };
+    __half2 sum = __floats2half2_rn(0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < kArray; i += 512) {
+      const uint4 w = load(v + i);
+      const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = __hfma2(h[j], __floats2half2_rn(0.f, 0.f), sum);
+    }
+    if (!__any_sync(0xffffffffu, __low2float(sum) != 0.f || __high2float(sum) != 0.f)) return false;
+    auto finite = [](uint32_t x) {
+      return ((x & 0x7c00u) == 0x7c00u ? 0u : x & 0xffffu) | ((x & 0x7c000000u) == 0x7c000000u ? 0u : x & 0xffff0000u);
+    };
+#pragma unroll 1
+    for (int i = 0; i < kArray; i += 512) {
+      const uint4 w = load(v + i);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v + i), "r"(finite(w.x)), "r"(finite(w.y)), "r"(finite(w.z)),
+                   "r"(finite(w.w)) : "memory");
+    }
+    __syncwarp();
+    return true;
+  }
+  // ... and join the rows that see them afterwards: z[key * kMaxNew + row] are their scores, -inf where masked.
+  __device__ __forceinline__ void add_wild(const CacheView& c, const NewTokens& nw, const float* z) {
+#pragma unroll 1
+    for (int k = 0; k < nw.nn; ++k) {
+      const int64_t slot = __shfl_sync(0xffffffffu, nw.slot, k);
+      if (slot < 0) continue;
+      const __half* v = static_cast<const __half*>(c.v) + slot * D + g;
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float x = __half2float(v[j * 16 + half * 8]);
+          if (fabsf(x) < kInf) continue;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const float s = z[k * kMaxNew + nt * 8 + 2 * t + q];
+              if (s != -kInf) o[j][nt][q + 2 * half] += x * ex2(s - m[nt][q]);
+            }
+        }
+    }
+  }
+
   template <bool kPrefix>
   __device__ __forceinline__ void run(const DecodeParams& p, const Job& job) {
     const CacheView& c = p.c;
@@ -481,6 +535,7 @@ struct MmaCore {
         for (int j = 0; j < MT; ++j) o[j][nt][q] = o[j][nt][q + 2] = 0.f;
       }
     float mid = later.finish(c, job.table, job.h);
+    bool wild = false;
     for (int i = 0; i < total; ++i) {
       copy_wait<kStages - 2>();
       __syncwarp();
@@ -550,11 +605,25 @@ struct MmaCore {
               z[sub][nt][key] = __fadd2_rn(make_float2(zz[0], zz[1]), ref[nt]);
             }
           }
+        if constexpr (!kPrefix && !kInt8) wild = clear_wild(st);
+        if (wild) {  // the pairs' place takes the scores (the newest tokens are the first 16 keys)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int key = 0; key < 2; ++key) {
+              float* at = pairs + (key * 8 + g) * kMaxNew + nt * 8 + 2 * t;
+              at[0] = z[0][nt][key].x - ref[nt].x;
+              at[1] = z[0][nt][key].y - ref[nt].y;
+            }
+        }
       }
       accumulate(st, z, rv);
       __syncwarp();
     }
     copy_wait<0>();
+    if constexpr (!kPrefix && !kInt8) {
+      if (wild) add_wild(c, nw, reinterpret_cast<const float*>(par));
+    }
   }
 
   __device__ __forceinline__ void store(float* sm, float* sl, float* sO, int rows) {

@@ -672,6 +672,62 @@ def test_int8_rows_near_the_end_of_float32():
         assert (scales[table[0, 0], :, :n].cpu().double() * 127 / top[..., 0] - 1).abs().max().item() <= 2.0 ** -22
 
 
+@pytest.mark.parametrize("dtype,storage", FORMS)
+@pytest.mark.parametrize("D,n,P", [(16, 5, 0), (64, 5, 0), (128, 16, 0), (256, 7, 0), (32, 2, 0), (64, 6, 300), (64, 9, 0)])
+def test_new_tokens_that_are_not_finite_stay_behind_the_mask(dtype, storage, D, n, P):
+    """A drafted token whose key, value or field is NaN or infinite does not reach the rows before it, which cannot see
+    it; what its value does to the other columns of the rows that see it is nothing either."""
+    H, L, page = 2, 70, 32
+    nan, inf = float("nan"), float("inf")
+    at = L - n + n // 2  # the token, and a later one for n > 2
+    cases = [("k", nan), ("k", inf), ("v", nan), ("v", inf), ("v", -inf), ("phi", nan), ("phi", -inf), ("psi", nan), ("psi", inf)]
+    B = len(cases)
+    q, k, v, phi, psi = sequence(B, H, L, D, dtype, seed=n)
+    names = dict(k=k, v=v, phi=phi, psi=psi)
+    for b, (name, value) in enumerate(cases):
+        if name in "kv":
+            names[name][b, :, at, 3] = value
+            names[name][b, :, L - 1, D - 1] = value
+        else:
+            names[name][b, :, at] = value
+    table, n_pages = tables([L] * B + [P], page)
+    table, ptable = table[:-1], table[-1, :-(-P // page)].contiguous()
+    cache = FPACache(n_pages, H, D, page, dtype, storage)
+    poison(cache)
+    kw, pre = {}, None
+    if P:
+        pre = [x[0] for x in sequence(1, H, P, D, dtype, 3)]
+        fill(cache, ptable[None], [P], *(x[None] for x in pre[1:]))
+        kw = dict(prefix_table=ptable, prefix_len=P)
+    fill(cache, table, [L] * B, k, v, phi, psi)
+    beta = torch.tensor([0.8, 1.3])
+    got = first_passage_decode(q[:, :, L - n:].cuda(), cache, table, i32([L] * B), beta.cuda(), **kw)
+    rows = at - (L - n)  # rows before the token
+    for b, (name, value) in enumerate(cases):
+        seq = [x[b, :, :at] for x in (q, k, v, phi, psi)]
+        if P:
+            seq = [torch.cat([x, y], 1) for x, y in zip(pre, seq)]
+        want = expected(*seq, beta, rows, storage)
+        assert torch.isfinite(got[b, :, :rows]).all(), (name, value)
+        assert_close(got[b, :, :rows], want, seq[2].abs().max().item(), dtype, (name, value))
+        if name == "v" and storage is None:
+            # The rows from it on: not finite in its column, as they were in the others.
+            rest = got[b, :, rows:n - 1].float().cpu()
+            assert not torch.isfinite(rest[..., 3]).any()
+            finite = v[b:b + 1, :, :].clone()
+            finite[0, :, at, 3] = finite[0, :, L - 1, D - 1] = 0
+            for r in range(rows, n - 1):
+                T = L - n + r + 1
+                seq = [x[b, :, :T] for x in (q, k)] + [finite[0, :, :T], phi[b, :, :T], psi[b, :, :T]]
+                if P:
+                    seq = [torch.cat([x, y], 1) for x, y in zip(pre, seq)]
+                want = expected(*seq, beta, 1, storage)[:, 0]
+                others = [d for d in range(D) if d != 3]
+                assert_close(got[b, :, r][:, others], want[:, others], seq[2].abs().max().item(), dtype, (name, value, r))
+        elif name in "kv" and not (storage is None and value == inf):  # an infinite product may be -inf, which is no weight
+            assert not torch.isfinite(got[b, :, rows:].float()).all(-1).any()
+
+
 def test_lengths_at_the_end_of_32_bits():
     """A table of 2^31 positions, all in one page: lengths end where rounding up to a page stays within 32 bits."""
     H, D, page = 1, 16, 256
