@@ -132,7 +132,8 @@ class LMGenerator:
 
     `extend(tokens)` runs the next n tokens of every sequence (at most 16 at a time after the first chunk) and returns
     their logits; `keep(counts)` says how many of them stay (refused drafts, or the padding of a ragged batch, are
-    simply written over by the next call). `generate` samples with or without a draft model.
+    simply written over by the next call). Tokens that `reset` made no room for are refused. `generate` samples with or
+    without a draft model, and raises what the kernels recorded in the caches' status words.
 
     dtype float16 runs the model under fp16 autocast, as training does, on the tensor-core kernels; float32 runs it as it
     is. storage=torch.int8 quantises the caches."""
@@ -149,11 +150,11 @@ class LMGenerator:
         """Start `batch` empty sequences with room for `tokens` tokens each, behind the tokens of `prefix` (a list, run
         once here) if given."""
         cfg = self.model.cfg
-        per, n_pre = -(-tokens // self.page), 0 if prefix is None else -(-len(prefix) // self.page)
+        per, n_pre = max(-(-tokens // self.page), 1), 0 if prefix is None else -(-len(prefix) // self.page)
         if n_pre + batch * per > self.n_pages:
             raise ValueError(f"the cache has {self.n_pages} pages, {n_pre + batch * per} are needed")
         i32 = dict(dtype=torch.int32, device=self.device)
-        self.prefix = {}
+        self.prefix, self._most = {}, 0  # _most: no sequence is longer (the lengths are on the device)
         if n_pre:
             self.table = torch.arange(n_pre, **i32)[None]
             self.lengths, self.walk = torch.zeros(1, **i32), torch.zeros(cfg.n_layers, 1, cfg.n_heads, device=self.device)
@@ -161,8 +162,8 @@ class LMGenerator:
             self.keep(torch.tensor([len(prefix)], **i32))
             walk, table = self.walk, self.table[0]
             self.prefix = dict(prefix_table=table, prefix_len=len(prefix))
-        self.table = n_pre + torch.arange(batch * max(per, 1), **i32).view(batch, max(per, 1))
-        self.lengths = torch.zeros(batch, **i32)
+        self.table = n_pre + torch.arange(batch * per, **i32).view(batch, per)
+        self.lengths, self._most = torch.zeros(batch, **i32), 0
         self.walk = walk.expand(-1, batch, -1).contiguous() if n_pre else \
             torch.zeros(cfg.n_layers, batch, cfg.n_heads, device=self.device)
 
@@ -183,6 +184,13 @@ class LMGenerator:
         m, (B, n) = self.model, tokens.shape
         if n > MAX_NEW_TOKENS and not first:
             raise ValueError(f"at most {MAX_NEW_TOKENS} tokens at a time")
+        room = self.table.shape[1] * self.page
+        if self._most + n > room or (first and self._most):
+            self._most = max(self.lengths.tolist(), default=0)  # waits for the device, when the bound is no longer enough
+        if self._most + n > room:
+            raise ValueError(f"{n} tokens after {self._most} exceed the room of {room} tokens")
+        if first and (self._most or self.prefix):
+            raise ValueError("first: only for empty sequences without a prefix")
         upto, walks = self.lengths + n, []
         with torch.autocast(device_type="cuda", dtype=torch.float16, enabled=self.dtype == torch.float16):
             x = m.wte(tokens)
@@ -204,6 +212,7 @@ class LMGenerator:
 
     def keep(self, counts):
         """The first counts[b] (int32) of the tokens of the last `extend` stay."""
+        self._most += self._walks.shape[2]
         self.lengths = self.lengths + counts
         w = torch.cat([self.walk[:, :, None], self._walks], 2)
         self.walk = w.gather(2, counts.long()[None, :, None, None].expand(w.shape[0], -1, 1, w.shape[3]))[:, :, 0]
@@ -270,4 +279,6 @@ class LMGenerator:
                 if len(x) < n_new:
                     x.extend(t for t in row if t >= 0)
             done = torch.tensor([len(x) >= n_new for x in out], device=self.device)
+        for cache in self.caches + (draft.caches if draft is not None else []):
+            cache.check()
         return [x[:n_new] for x in out]

@@ -122,3 +122,55 @@ def test_refusals():
         gen.extend(torch.zeros(1, 17, dtype=torch.long, device="cuda"))
     with pytest.raises(ValueError, match="no prompt may be empty"):
         gen.generate([[]], 1)
+
+
+def test_tokens_past_the_room_are_refused():
+    """What `reset` has given no room for is refused, by the lengths as they are and not by what was fed and taken back."""
+    gen = LMGenerator(model(), 200, page_size=32, dtype=F32)
+    tokens = torch.zeros(2, 16, dtype=torch.long, device="cuda")
+    for prefix in (None, list(range(40))):
+        gen.reset(2, 60, prefix)  # two pages of 32 each
+        for i in range(30):       # far more than 64 tokens, all taken back
+            gen.extend(tokens)
+            gen.keep(torch.zeros(2, dtype=torch.int32, device="cuda"))
+        for _ in range(3):
+            gen.extend(tokens)
+            gen.keep(torch.tensor([5, 16], dtype=torch.int32, device="cuda"))
+        gen.extend(tokens)
+        gen.keep(torch.tensor([16, 15], dtype=torch.int32, device="cuda"))
+        gen.extend(tokens[:, :1])
+        with pytest.raises(ValueError, match="room"):
+            gen.extend(tokens[:, :2])
+    gen.reset(2, 60)
+    with pytest.raises(ValueError, match="room"):
+        gen.extend(torch.zeros(2, 65, dtype=torch.long, device="cuda"), first=True)
+    gen.reset(2, 60)
+    gen.extend(tokens)
+    gen.keep(torch.ones(2, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="first"):
+        gen.extend(tokens, first=True)
+    gen.reset(2, 60, [1, 2, 3])
+    with pytest.raises(ValueError, match="first"):
+        gen.extend(tokens, first=True)
+    with pytest.raises(ValueError, match="pages"):
+        gen.reset(8, 0)  # each sequence holds a page
+    for c in gen.caches:
+        c.check()
+
+
+def test_generate_raises_what_the_kernels_report():
+    """A page id outside the pool, met while answering: no answer comes back."""
+    for which in (0, 1):
+        gen = LMGenerator(model(), 1000, page_size=32, dtype=F32)
+        draft = LMGenerator(model(seed=2), 1000, page_size=32, dtype=F32)
+        bad = (gen, draft)[which]
+        start = bad._start
+
+        def broken(*args):
+            cur = start(*args)
+            bad.table[0, 0] = 10 ** 6
+            return cur
+
+        bad._start = broken
+        with pytest.raises(ValueError, match="outside"):
+            gen.generate([[1, 2, 3], [4, 5]], 6, draft=draft, n_draft=2)
