@@ -211,7 +211,8 @@ class LMGenerator:
             return F.linear(m.ln_f(x), m.wte.weight).float()
 
     def keep(self, counts):
-        """The first counts[b] (int32) of the tokens of the last `extend` stay."""
+        """The first counts[b] (int32) of the tokens of the last `extend` stay; at most all of them."""
+        counts = counts.clamp(0, self._walks.shape[2])
         self._most += self._walks.shape[2]
         self.lengths = self.lengths + counts
         w = torch.cat([self.walk[:, :, None], self._walks], 2)

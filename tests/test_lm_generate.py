@@ -174,3 +174,17 @@ def test_generate_raises_what_the_kernels_report():
         bad._start = broken
         with pytest.raises(ValueError, match="outside"):
             gen.generate([[1, 2, 3], [4, 5]], 6, draft=draft, n_draft=2)
+
+
+def test_keep_takes_no_more_than_was_fed():
+    """Counts outside 0 .. n: an index past the walks would be a fault on the device."""
+    gen = LMGenerator(model(), 400, page_size=32, dtype=F32)
+    tokens = torch.arange(12, device="cuda").view(3, 4)
+    walks = []
+    for counts in ([4, 0, 2], [2 ** 31 - 1, -5, 2]):
+        gen.reset(3, 60)
+        gen.extend(tokens)
+        gen.keep(torch.tensor(counts, dtype=torch.int32, device="cuda"))
+        assert gen.lengths.tolist() == [4, 0, 2]
+        walks.append(gen.walk)
+    assert torch.equal(*walks)
