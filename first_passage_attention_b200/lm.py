@@ -158,7 +158,7 @@ class LMGenerator:
         if n_pre:
             self.table = torch.arange(n_pre, **i32)[None]
             self.lengths, self.walk = torch.zeros(1, **i32), torch.zeros(cfg.n_layers, 1, cfg.n_heads, device=self.device)
-            self.extend(torch.tensor([list(prefix)], device=self.device), first=True)
+            self.extend(torch.tensor([list(prefix)], device=self.device), first=True, logits=False)
             self.keep(torch.tensor([len(prefix)], **i32))
             walk, table = self.walk, self.table[0]
             self.prefix = dict(prefix_table=table, prefix_len=len(prefix))
@@ -177,10 +177,10 @@ class LMGenerator:
             return (w + out[:, :, 1]).transpose(1, 2), (w + out[:, :, 2]).transpose(1, 2), w
 
     @torch.no_grad()
-    def extend(self, tokens, first=False):
+    def extend(self, tokens, first=False, logits=True):
         """Logits [B, n, vocab] of the next tokens [B, n] of every sequence, which enter the caches at `lengths`.
         first: the sequences are empty and there is no prefix; n may then exceed 16, and the tokens attend to each
-        other through the training kernels."""
+        other through the training kernels. logits False: fill the caches only, and return None."""
         m, (B, n) = self.model, tokens.shape
         if n > MAX_NEW_TOKENS and not first:
             raise ValueError(f"at most {MAX_NEW_TOKENS} tokens at a time")
@@ -208,7 +208,7 @@ class LMGenerator:
                 x = x + blk.mlp(blk.ln2(x))
                 walks.append(w)
             self._walks = torch.stack(walks)  # [layers, B, n, H]
-            return F.linear(m.ln_f(x), m.wte.weight).float()
+            return F.linear(m.ln_f(x), m.wte.weight).float() if logits else None
 
     def keep(self, counts):
         """The first counts[b] (int32) of the tokens of the last `extend` stay; at most all of them."""
@@ -225,12 +225,12 @@ class LMGenerator:
         T = max(len(p) for p in prompts) - 1
         padded = torch.tensor([list(p[:-1]) + [0] * (T - len(p) + 1) for p in prompts], device=self.device)
         if T and not self.prefix:
-            self.extend(padded, first=True)
+            self.extend(padded, first=True, logits=False)
             self.keep(lens)
         elif T:
             for i in range(0, T, MAX_NEW_TOKENS):
                 part = padded[:, i:i + MAX_NEW_TOKENS]
-                self.extend(part)
+                self.extend(part, logits=False)
                 self.keep((lens - i).clamp(0, part.shape[1]).int())
         return torch.tensor([p[-1] for p in prompts], device=self.device)
 

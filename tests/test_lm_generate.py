@@ -188,3 +188,18 @@ def test_keep_takes_no_more_than_was_fed():
         assert gen.lengths.tolist() == [4, 0, 2]
         walks.append(gen.walk)
     assert torch.equal(*walks)
+
+
+def test_feeding_a_prompt_needs_no_logits():
+    """Prompts and prefixes go into the caches without the output layer's [tokens, vocabulary] logits."""
+    cfg = LMConfig(vocab=50304, d_model=64, n_heads=2, n_layers=1)
+    gen = LMGenerator(model(cfg), 8000, page_size=64)
+    g = torch.Generator().manual_seed(7)
+    ids = torch.randint(0, cfg.vocab, (3000,), generator=g).tolist()
+    torch.cuda.synchronize()
+    for prompts, prefix in (([ids[:1500], ids[1500:]], None), ([ids[:40]], ids)):
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        gen.generate(prompts, 2, prefix=prefix)
+        # The logits of one chunk of 16 tokens in fp16 and float32 are 5 MB, those of 3000 tokens 900 MB.
+        assert torch.cuda.max_memory_allocated() - before < 100 * 2 ** 20
