@@ -243,6 +243,12 @@ class LMGenerator:
             n_draft = 0
         if not 0 <= n_draft < MAX_NEW_TOKENS or any(len(p) == 0 for p in prompts):
             raise ValueError(f"n_draft must lie below {MAX_NEW_TOKENS}, and no prompt may be empty")
+        if not prompts:
+            raise ValueError("at least one prompt")
+        if not temperature > 0:
+            raise ValueError("the temperature must be positive")
+        if draft is self:
+            raise ValueError("the draft needs caches of its own (another LMGenerator; the model may be the same)")
         B, room = len(prompts), n_new + 2 * n_draft + 2
         cur = self._start(prompts, room, prefix)
         if draft is not None:

@@ -203,3 +203,14 @@ def test_feeding_a_prompt_needs_no_logits():
         gen.generate(prompts, 2, prefix=prefix)
         # The logits of one chunk of 16 tokens in fp16 and float32 are 5 MB, those of 3000 tokens 900 MB.
         assert torch.cuda.max_memory_allocated() - before < 100 * 2 ** 20
+
+
+def test_generate_refusals():
+    gen = LMGenerator(model(), 1000, page_size=32, dtype=F32)
+    for temperature in (0.0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            gen.generate([[1]], 2, temperature=temperature)
+    with pytest.raises(ValueError, match="draft"):
+        gen.generate([[1]], 2, draft=gen)
+    with pytest.raises(ValueError, match="prompt"):
+        gen.generate([], 2)
