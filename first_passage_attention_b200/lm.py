@@ -150,6 +150,7 @@ class LMGenerator:
         """Start `batch` empty sequences with room for `tokens` tokens each, behind the tokens of `prefix` (a list, run
         once here) if given."""
         cfg = self.model.cfg
+        self._check_ids(prefix or [])
         per, n_pre = max(-(-tokens // self.page), 1), 0 if prefix is None else -(-len(prefix) // self.page)
         if n_pre + batch * per > self.n_pages:
             raise ValueError(f"the cache has {self.n_pages} pages, {n_pre + batch * per} are needed")
@@ -166,6 +167,11 @@ class LMGenerator:
         self.lengths, self._most = torch.zeros(batch, **i32), 0
         self.walk = walk.expand(-1, batch, -1).contiguous() if n_pre else \
             torch.zeros(cfg.n_layers, batch, cfg.n_heads, device=self.device)
+
+    def _check_ids(self, ids):
+        # On the device an id outside the embedding is a fault that ends the process.
+        if any(not 0 <= t < self.model.cfg.vocab for t in ids):
+            raise ValueError(f"token ids must lie in [0, {self.model.cfg.vocab})")
 
     def _field(self, field, x, walk):
         """The layer's field of the next tokens (`Field` starts its walk at 0): phi, psi [B, H, n], and the walk
@@ -245,6 +251,10 @@ class LMGenerator:
             raise ValueError(f"n_draft must lie below {MAX_NEW_TOKENS}, and no prompt may be empty")
         if not prompts:
             raise ValueError("at least one prompt")
+        for p in prompts:
+            self._check_ids(p)
+        if draft is not None and draft.model.cfg.vocab != self.model.cfg.vocab:
+            raise ValueError("the draft's vocabulary must be the model's")
         if not temperature > 0:
             raise ValueError("the temperature must be positive")
         if draft is self:

@@ -214,3 +214,20 @@ def test_generate_refusals():
         gen.generate([[1]], 2, draft=gen)
     with pytest.raises(ValueError, match="prompt"):
         gen.generate([], 2)
+
+
+def test_ids_outside_the_vocabulary_are_refused():
+    """Raised on the host: on the device they would be faults."""
+    gen = LMGenerator(model(), 1000, page_size=32, dtype=F32)
+    for bad in (-1, CFG.vocab):
+        with pytest.raises(ValueError, match="token ids"):
+            gen.generate([[1, 2], [3, bad]], 2)
+        with pytest.raises(ValueError, match="token ids"):
+            gen.generate([[1, 2]], 2, prefix=[0, bad])
+        with pytest.raises(ValueError, match="token ids"):
+            gen.reset(1, 32, [bad])
+    for vocab in (CFG.vocab - 1, CFG.vocab + 64):
+        draft = LMGenerator(model(LMConfig(vocab=vocab, d_model=64, n_heads=2, n_layers=1)), 1000, page_size=32, dtype=F32)
+        with pytest.raises(ValueError, match="vocabulary"):
+            gen.generate([[1, 2]], 2, draft=draft)
+    assert len(gen.generate([[1, CFG.vocab - 1]], 3, prefix=[0])[0]) == 3
