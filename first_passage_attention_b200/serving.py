@@ -1,5 +1,6 @@
 """Serving a model with First Passage Attention: the paged cache, attention of the newest tokens over it, and the
-verification of drafted tokens. Forward only; every call runs the native kernels of libfpa_b200 on the current stream,
+verification of drafted tokens. Forward only (tensors that require grad are refused while gradients are recorded); every
+call runs the native kernels of libfpa_b200 on the current stream,
 allocates its outputs only, never synchronises, and can be captured in a CUDA graph.
 
 ``FPACache`` holds keys, values and the field of many sequences in pages of a common pool, as the model's fp16 or fp32
@@ -29,6 +30,12 @@ _HEAD_DIMS = (16, 32, 64, 128, 256)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _refuse_grad(what):
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} is forward only and no gradient would reach its inputs: call it under torch.no_grad() "
+                           "or with detached tensors")
 
 
 def _int32_on(name, x, index, n):
@@ -128,6 +135,8 @@ class FPACache:
         dev = self._index
         if k.get_device() != dev or v.get_device() != dev or phi.get_device() != dev or psi.get_device() != dev:
             raise ValueError(f"k, v, phi and psi must be on the cache's device cuda:{dev}")
+        if k.requires_grad or v.requires_grad or phi.requires_grad or psi.requires_grad:
+            _refuse_grad("FPACache.append")
         if B == 0 or n == 0:
             return
         a = _lib.FpaAppendArgs()
@@ -188,6 +197,8 @@ def first_passage_decode(q, cache, block_table, lengths, beta, prefix_table=None
         raise ValueError(f"q must be {cache.dtype} on {cache.device}")
     if beta.shape != (H,) or beta.dtype != torch.float32 or beta.get_device() != dev or not beta.is_contiguous():
         raise ValueError(f"beta must be a contiguous float32 tensor of shape ({H},) on {cache.device}")
+    if q.requires_grad or beta.requires_grad:
+        _refuse_grad("first_passage_decode")
     pages, ptable = 0, 0
     if prefix_len < 0 or (prefix_len > 0 and prefix_table is None):
         raise ValueError("prefix_len must not be negative, and needs a prefix_table")

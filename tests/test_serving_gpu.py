@@ -745,6 +745,23 @@ def test_lengths_at_the_end_of_32_bits():
                 cache.check()
 
 
+def test_gradients_are_refused_not_lost():
+    """Forward only: a tensor that wants a gradient is refused while gradients are recorded."""
+    cache = FPACache(4, 2, 32, 32)
+    t, n, beta = i32([[0, 1]]), i32([1]), torch.ones(2, device="cuda")
+    x = torch.zeros(1, 2, 1, 32, dtype=F16, device="cuda")
+    f = torch.zeros(1, 2, 1, device="cuda")
+    leaf = lambda y: y.clone().requires_grad_()  # noqa: E731
+    cache.append(x, x, f, f, t, i32([0]))
+    for call in (lambda: first_passage_decode(leaf(x), cache, t, n, beta), lambda: first_passage_decode(x, cache, t, n, leaf(beta)),
+                 lambda: cache.append(leaf(x), x, f, f, t, i32([0])), lambda: cache.append(x, leaf(x), f, f, t, i32([0])),
+                 lambda: cache.append(x, x, leaf(f), f, t, i32([0])), lambda: cache.append(x, x, f, leaf(f), t, i32([0]))):
+        with pytest.raises(RuntimeError, match="forward only"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 # ------------------------------------------------------------------------------------------------ verification ----
 
 def verify_oracle(p, q, draft, u, noise, lens=None):
