@@ -293,6 +293,25 @@ def test_decode_in_two_launches(B, H, n, D, dtype, storage, P):
     assert all(torch.equal(x, y[0]) for y in outs for x in y) and not torch.equal(outs[0][0], outs[1][0])
 
 
+@pytest.mark.parametrize("B,H,n,D,storage,P", [(40, 16, 1, 32, None, 0), (40, 16, 2, 64, I8, 0), (40, 16, 2, 128, None, 0), (55, 12, 2, 32, None, 50)])
+def test_float32_decode_in_two_launches(B, H, n, D, storage, P):
+    """As above, for float32 queries: 592 places (296 at D = 128) and a few sequences more than a round of them holds."""
+    lens = [min(i * 37 % 150, 101) for i in range(B - 3)] + [1030, 3, 640]
+    cache, table, qn, beta, got, kw = run_decode(lens, n, H, D, 64, F32, storage, seed=B, P=P)
+    q, lengths, beta = qn.cuda(), i32(lens), beta.cuda()
+    LaunchStats.reset()
+    assert torch.equal(first_passage_decode(q, cache, table, lengths, beta, **kw), got)
+    assert LaunchStats.kernels == (4 if P else 2)
+    last = i32([max(x - 1, 0) for x in lens])
+    _, k, v, phi, psi = (x.cuda() for x in sequence(B, H, 2, D, F32, seed=9))
+    outs = [[], []]
+    for i in range(20):
+        j = i & 1
+        cache.append(k[:, :, j:j + 1], v[:, :, j:j + 1], phi[..., j:j + 1], psi[..., j:j + 1], table, last, (lengths > 0).int())
+        outs[j].append(first_passage_decode(q, cache, table, lengths, beta, **kw))
+    assert all(torch.equal(x, y[0]) for y in outs for x in y) and not torch.equal(outs[0][0], outs[1][0])
+
+
 @pytest.mark.parametrize("beta", [-0.7, 0.0, 3.0])
 @pytest.mark.parametrize("dtype,storage", [(F16, I8), (F32, None)])
 def test_decode_beta_and_wide_fields(beta, dtype, storage):
