@@ -155,11 +155,8 @@ struct FfmaCore {
     }
   }
 
-  // O += P V of the eight keys in stage i, columns first .. first + 7 of P. kMasked: some rows do not see all of these keys;
-  // what they do not see stays out of their sums even where it is not finite.
-  template <bool kMasked>
+  // O += P V of the eight keys in stage i, columns first .. first + 7 of P.
   __device__ __forceinline__ void values(int i, int first) {
-    auto add = [](float e, float v, float x) { return kMasked && e == 0.f ? x : fmaf(e, v, x); };
     const char* rows = ring_ptr + (i % kStages) * kStage;
     if constexpr (KG > 1) {
 #pragma unroll
@@ -168,7 +165,7 @@ struct FfmaCore {
         float v[CPL];
         load_v(rows + k * kPitch, v);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) o[r][0] = add(ss[r * 32 + first + k], v[0], o[r][0]);
+        for (int r = 0; r < NR; ++r) o[r][0] = fmaf(ss[r * 32 + first + k], v[0], o[r][0]);
       }
     } else {
 #pragma unroll
@@ -182,12 +179,30 @@ struct FfmaCore {
 #pragma unroll
           for (int j = 0; j < CPL; ++j) {
             float x = o[r][j];
-            x = add(e.x, v[0][j], x);
-            x = add(e.y, v[1][j], x);
-            x = add(e.z, v[2][j], x);
-            o[r][j] = add(e.w, v[3][j], x);
+            x = fmaf(e.x, v[0][j], x);
+            x = fmaf(e.y, v[1][j], x);
+            x = fmaf(e.z, v[2][j], x);
+            o[r][j] = fmaf(e.w, v[3][j], x);
           }
         }
+      }
+    }
+  }
+
+  // The same for the newest tokens, n of them in the tile. Some rows do not see all of these keys: what they do not see stays
+  // out of their sums even where it is not finite.
+  __device__ __forceinline__ void values_new(int i, int first, int n) {
+    const char* rows = ring_ptr + (i % kStages) * kStage;
+#pragma unroll 1
+    for (int k0 = 0; k0 < min(8, n - first); k0 += KG) {
+      const int k = k0 + (KG > 1 ? lane / D : 0);
+      float v[CPL];
+      load_v(rows + k * kPitch, v);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float e = ss[r * 32 + first + k];
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) o[r][j] = e == 0.f ? o[r][j] : fmaf(e, v[j], o[r][j]);
       }
     }
   }
@@ -318,9 +333,9 @@ struct FfmaCore {
       for (int j = 0; j < 4; ++j) {
         next(8 * k + 4 + j);
         if (fresh)
-          values<true>(8 * k + 4 + j, j * 8);
+          values_new(8 * k + 4 + j, j * 8, job.n_new);
         else
-          values<false>(8 * k + 4 + j, j * 8);
+          values(8 * k + 4 + j, j * 8);
       }
     }
     copy_wait<0>();
