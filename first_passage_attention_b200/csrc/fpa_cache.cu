@@ -23,7 +23,8 @@ constexpr int kReadThreads = 128;
 constexpr int kMaxThreads = 256;
 constexpr int kAhead = 4;  // rows whose loads a thread has in flight
 
-// Codes + 128 of eight elements from their row's largest magnitude, four to a word.
+// Codes + 128 of eight elements of type T from their row's largest magnitude, four to a word.
+template <typename T>
 __device__ __forceinline__ uint2 encode8(const float (&x)[8], float top) {
   constexpr float kRound = 12582912.f + 128.f;  // 1.5 2^23: a sum with it is rounded to an integer, even on ties
   const float k = 127.f * rcp_approx_f(top);
@@ -40,11 +41,10 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8], float top) {
   }
   // Near a half, or the reciprocal leaves float32's normal range, or NaN (codes 0).
   if (!(off < 0.5f - 0x1p-14f) || !(top < 0x1p100f)) {
-    // 127 x would leave float32 for the largest rows: those are scaled down, which is exact where it matters.
-    const float down = top < 0x1p100f ? 1.f : 0x1p-20f;
+    // 127 x would leave float32 for its largest rows: both sides are scaled down there, which is exact where it matters.
+    const float down = sizeof(T) == 2 || top < 0x1p100f ? 1.f : 0x1p-20f, t = top * down;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      w[j] = min(max(__float2int_rn(__fdiv_rn(__fmul_rn(x[j] * down, 127.f), top * down)), -127), 127) + 128;
+    for (int j = 0; j < 8; ++j) w[j] = min(max(__float2int_rn(__fdiv_rn(__fmul_rn(x[j], 127.f * down), t)), -127), 127) + 128;
   }
   auto four = [&](int j) {
     return __byte_perm(__byte_perm(w[j], w[j + 1], 0x0040), __byte_perm(w[j + 2], w[j + 3], 0x0040), 0x5410);
@@ -117,9 +117,10 @@ struct AppendParams {
   const int32_t* counts;
 };
 
-// T: type of k and v; kInt8: codes and scales, else rows as they are.
+// T: type of k and v; kInt8: codes and scales, else rows as they are. Four blocks on an SM, three for codes from float32, whose
+// registers would spill (16 x 12 pairs of up to 2048 tokens of 64: 50 us with four, 42 with three).
 template <typename T, bool kInt8>
-__global__ void __launch_bounds__(kMaxThreads, 4) append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kMaxThreads, kInt8 && sizeof(T) == 4 ? 3 : 4) append_kernel(const __grid_constant__ AppendParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const CacheView& c = p.c;
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(kMaxThreads, 4) append_kernel(const __grid_con
         // zeros takes that smallest scale, so that it does not outweigh small rows there. A row with a NaN or an infinity
         // has no codes: its scale is NaN.
         top[a] = m < kInf ? fmaxf(m, 127.f * 0x1p-90f) : __int_as_float(0x7fffffff);
-        const uint2 w = encode8(x[a], top[a]);
+        const uint2 w = encode8<T>(x[a], top[a]);
         if (ok) *reinterpret_cast<uint2*>(dst + a * dst_step) = w;
       } else if (ok) {
         store8(reinterpret_cast<T*>(dst + a * dst_step), x[a]);
