@@ -294,7 +294,8 @@ struct FfmaCore {
     };
     for (int k = 0; k < total; ++k) {
       // The tile's field, before the fetches go on to the next tile's.
-      const bool fresh = k >= history, ok = fresh ? nw.slot >= 0 : lane < lim;
+      // (A single row has no such tile: its own key is the history's last.)
+      const bool fresh = NR > 1 && k >= history, ok = fresh ? nw.slot >= 0 : lane < lim;
       float f_phi = phi, f_psi = psi, f_ks = ks, f_vs = vs;
       if (fresh) {
         f_ks = f_vs = 0.f;
