@@ -10,9 +10,11 @@
 // at a quarter of the rate. Stored is code + 128. A block of the append owns one page of one (sequence, head): it alone
 // writes the page's minimum of phi.
 //
-// On a B200: 8 x 16 (sequence, head) pairs of 16383 int8 tokens of 128 read back as fp16 in 230 us, 6.3 TB/s; 64 x 12
-// pairs of up to 2048 fp16 tokens of 64 appended as int8 in 181 us, 2.3 TB/s, bound by about 13 instructions for an element; 4 x
-// 16 of 16383 fp16 tokens of 128 as they are in 156 us; 32 x 12 single tokens in 3.5 us.
+// On a B200: 8 x 16 (sequence, head) pairs of 16383 int8 tokens of 128 read back as fp16 in 230 us, 6.3 TB/s, and fp16 tokens
+// (up to 16383) as they are in 316 us, 5.9 TB/s; 64 x 12 pairs of up to 2048 fp16 tokens of 64 appended as int8 in 184 us,
+// 2.3 TB/s, where neither pipe is full (issue slots 54 %, HBM 26 % of nominal, 46 % of the warps): at this page size a block
+// loads its rows once, converts them and stores them, and the wait for the loads is not covered; 4 x 16 of up to 16383 fp16
+// tokens of 128 as they are in 183 us, 4.7 TB/s; 32 x 12 single tokens in 3.5 us.
 #include "fpa_serve.h"
 #include "fpa_sm100.cuh"
 

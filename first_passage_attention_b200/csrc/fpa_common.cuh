@@ -53,9 +53,13 @@ __device__ __forceinline__ float lg2(float x) {
 // kernel before it on the stream is still running, once every CTA of that kernel has called pdl_launch_dependents
 // (or exited): its CTAs run their prologue (shared-memory carving, barrier set-up, TMEM allocation), then
 // pdl_wait() blocks until the previous kernel has completed and its memory writes are visible. Every kernel
-// launched that way calls pdl_wait() before its first global-memory access, and pdl_launch_dependents() only after
-// it, so that no more than two kernels of a stream overlap. Both are no-ops for a kernel launched without the
-// attribute.
+// launched that way writes to global memory only after pdl_wait(), and completes only after it (some of its threads
+// wait), so that the kernels of a stream complete in order. Nearly all call it before their first access, and
+// pdl_launch_dependents() only after it, so that no more than two kernels of a stream overlap. The exceptions are inside
+// one serving call: the first kernel of fpa_decode waits for whatever wrote the caller's tensors before it lets the next
+// one start, so the kernels behind it read those tensors before they wait, and wait where they read each other's results
+// (fpa_prefix_tc.cu, fpa_decode.cuh); the first of two decode launches behind a prefix lets the second start before it
+// waits, and three kernels can then overlap. Both calls are no-ops for a kernel launched without the attribute.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -16,9 +16,9 @@
 // head. The softmax states (m, l, O) of the warps join in shared memory, those of the cluster's CTAs through
 // distributed shared memory: no atomics, a fixed order, one launch (two where a last round would stay mostly empty).
 //
-// On a B200, whole calls in a graph: 4 x 16 pairs of 16383 fp16 tokens of 128, 5 rows, 64 us, 5.5 TB/s; 64 x 12 of up to 2048
-// tokens of 64, one row, fp16 36 us, int8 33 us, 4.4 TB/s; 12 heads of 1000 fp16 tokens 6.7 us; float32, 8 x 8 of
-// 1000 tokens of 32, 3 rows, 12.8 us.
+// On a B200, whole calls in a graph: 4 x 16 pairs of up to 16383 fp16 tokens of 128, 5 rows, 65 us, 5.5 TB/s; 64 x 12 of up to
+// 2048 tokens of 64, one row, over the same lengths in fp16 45.6 us, 6.0 TB/s, and in int8 32.7 us, 4.5 TB/s; 12 heads of
+// 1000 fp16 tokens 6.7 us; float32, 8 x 8 of up to 1000 tokens of 32, 3 rows, 13 us.
 #pragma once
 
 #include "fpa_serve.h"

@@ -17,7 +17,7 @@
 // whatever they hold, and because codes have to be converted on the way. Warp 16: the MMAs. Warps 17 and 18: the keys'
 // field and scales, alternate tiles. Every wait is bounded.
 //
-// On a B200: 120 rows behind 16383 fp16 tokens, 16 heads of 128, 40 us (430 TFLOP/s; 3.2k cycles for a tile of 128 keys); 64 rows
+// On a B200: 120 rows behind 16383 fp16 tokens, 16 heads of 128, 40 us (403 TFLOP/s; 3.2k cycles for a tile of 128 keys); 64 rows
 // behind 8192 int8 tokens, 12 heads of 64, 16 us, of which 11 are the CTA's start and end.
 #include <cuda_fp16.h>
 
