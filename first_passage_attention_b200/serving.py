@@ -1,7 +1,7 @@
 """Serving a model with First Passage Attention: the paged cache, attention of the newest tokens over it, and the
 verification of drafted tokens. Forward only (tensors that require grad are refused while gradients are recorded); every
-call runs the native kernels of libfpa_b200 on the current stream,
-allocates its outputs only, never synchronises, and can be captured in a CUDA graph.
+call runs the native kernels of libfpa_b200 on the current stream, allocates its outputs only, never synchronises, and can
+be captured in a CUDA graph.
 
 ``FPACache`` holds keys, values and the field of many sequences in pages of a common pool, as the model's fp16 or fp32
 values or as int8 codes with a scale for each token and head. A sequence's position s lies in page
